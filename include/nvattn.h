@@ -425,6 +425,60 @@ NVATTN_API nvattn_status nvattn_paged_prefill_rows(
     const uint16_t* k_rows_f16_dev, const uint16_t* v_rows_f16_dev, float* out_dev,
     nvattn_stream_t stream);
 
+/* ---- 8-bit paged KV cache ------------------------------------------------ */
+
+/* An alternative to the BF16 cache at about half its size (264 instead of 512
+ * bytes per token and kv head); the reference has no counterpart.  K and V
+ * each take two device arrays that the caller allocates:
+ *   payload [n_layer][num_blocks][n_kv_heads][block_size][head_dim] e4m3 bytes
+ *   scale   [n_layer][num_blocks][n_kv_heads][block_size] f32
+ * (block ids, block tables and slots as in the BF16 cache; inside a block the
+ * heads are outermost, so one head's block is contiguous).  A row x of 128
+ * values is held as e4m3(x / s) under s = 2^E, the smallest power of two with
+ * max|x| <= 448 s (E >= -100; s = 1 for a row of zeros), rounded to nearest
+ * even; payload * s, the value every reader uses, is exact in bf16.  A row
+ * that holds a NaN or an infinity is stored under a NaN scale and reads back
+ * as NaN throughout. */
+
+/* nvattn_kv_store_qk_norm_rope into the 8-bit cache: the same norm, rotation,
+ * q_out and, where k_rows_f16_dev / v_rows_f16_dev are given (both or
+ * neither), the same f16 rows (of the values before rounding to 8 bits) as
+ * nvattn_kv_store_qk_norm_rope_rows.  The slots >= 0 of one call are distinct
+ * (a slot named twice is left holding a mix of its rows). */
+NVATTN_API nvattn_status nvattn_kv_store_q8(
+    nvattn_handle* h, int layer, int n_tokens, const float* q_dev, const float* k_dev,
+    const float* v_dev, const uint16_t* q_norm_w_dev, const uint16_t* k_norm_w_dev,
+    const int32_t* positions_dev, const int32_t* slot_mapping_dev, void* q_out_dev,
+    nvattn_dtype q_out_dtype, uint8_t* k_q8_dev, float* k_scale_dev, uint8_t* v_q8_dev,
+    float* v_scale_dev, uint16_t* k_rows_f16_dev, uint16_t* v_rows_f16_dev,
+    nvattn_stream_t stream);
+
+/* Reads the rows of n_tokens slots back (a slot may be named more than once):
+ *   k_out_dev, v_out_dev [n_tokens][n_kv_heads][head_dim] in out_dtype
+ * bf16 and f32 exactly; f16 rounded to nearest even (overflow to infinity).
+ * A slot < 0 gives a row of zeros; a slot outside the cache too, and is
+ * reported.  In bf16 the rows have the BF16 cache's layout, so the slots of a
+ * block read into a BF16 cache's block make a prefix that
+ * nvattn_paged_prefill(_rows) can attend. */
+NVATTN_API nvattn_status nvattn_kv_load_q8(
+    nvattn_handle* h, int layer, int n_tokens, const int32_t* slot_mapping_dev,
+    const uint8_t* k_q8_dev, const float* k_scale_dev, const uint8_t* v_q8_dev,
+    const float* v_scale_dev, nvattn_dtype out_dtype, void* k_out_dev, void* v_out_dev,
+    nvattn_stream_t stream);
+
+/* nvattn_paged_decode over the 8-bit cache.  q_dev and out_dev are
+ * [n_seqs][n_q_heads][head_dim] in dtype, f32 or bf16 (sums in f32 either
+ * way; queries and softmax weights carry 22 bits).  Slots behind a sequence's
+ * context may hold anything.  A sequence of length 0 gives zeros.
+ * The launch uses the handle's workspace: calls on one handle are issued on
+ * one stream, as for nvattn_paged_decode. */
+NVATTN_API nvattn_status nvattn_paged_decode_q8(
+    nvattn_handle* h, int layer, int n_seqs, const void* q_dev, nvattn_dtype dtype,
+    const uint8_t* k_q8_dev, const float* k_scale_dev, const uint8_t* v_q8_dev,
+    const float* v_scale_dev, const int32_t* block_tables_dev, int max_blocks,
+    const int32_t* context_lens_dev, int max_context_len, void* out_dev,
+    nvattn_stream_t stream);
+
 /* ---- decode without any allocation -------------------------------------- */
 
 /* Where a kernel records the first error it meets (device memory owned by

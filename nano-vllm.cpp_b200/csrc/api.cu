@@ -70,16 +70,30 @@ nvattn_status encode_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t 
   return r == CUDA_SUCCESS ? NVATTN_OK : NVATTN_ERR_CUDA;
 }
 
+namespace {
+// Adds an entry to the handle's descriptor cache, round-robin once it is full.
+void keep_tensor_map(nvattn_handle* h, const NvattnTensorMapEntry& e) {
+  int slot;
+  if (h->n_maps < nvattn_handle::kMapCacheSize) {
+    slot = h->n_maps++;
+  } else {
+    slot = h->next_map;
+    h->next_map = (h->next_map + 1) % nvattn_handle::kMapCacheSize;
+  }
+  h->maps[slot] = e;
+}
+}  // namespace
+
 nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d, int box_rows,
                                    int swizzle, CUtensorMap* out) {
   for (int i = 0; i < h->n_maps; ++i) {
     const NvattnTensorMapEntry& e = h->maps[i];
-    if (e.base == base && e.box_d == box_d && e.box_rows == box_rows && e.swizzle == swizzle) {
+    if (!e.q8 && e.base == base && e.box_d == box_d && e.box_rows == box_rows && e.swizzle == swizzle) {
       *out = e.map;
       return NVATTN_OK;
     }
   }
-  NvattnTensorMapEntry e;
+  NvattnTensorMapEntry e = {};
   e.base = base;
   e.box_d = box_d;
   e.box_rows = box_rows;
@@ -90,14 +104,32 @@ nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d
                                           Hkv * D * 2, (uint32_t)box_d, 1, (uint32_t)box_rows,
                                           swizzle);
   if (st != NVATTN_OK) return st;
-  int slot;
-  if (h->n_maps < nvattn_handle::kMapCacheSize) {
-    slot = h->n_maps++;
-  } else {
-    slot = h->next_map;
-    h->next_map = (h->next_map + 1) % nvattn_handle::kMapCacheSize;
+  keep_tensor_map(h, e);
+  *out = e.map;
+  return NVATTN_OK;
+}
+
+nvattn_status get_q8_tensor_map(nvattn_handle* h, const void* base, int box_rows,
+                                CUtensorMap* out) {
+  for (int i = 0; i < h->n_maps; ++i) {
+    const NvattnTensorMapEntry& e = h->maps[i];
+    if (e.q8 && e.base == base && e.box_rows == box_rows) {
+      *out = e.map;
+      return NVATTN_OK;
+    }
   }
-  h->maps[slot] = e;
+  NvattnTensorMapEntry e = {};
+  e.base = base;
+  e.box_rows = box_rows;
+  e.q8 = true;
+  const uint64_t D = (uint64_t)h->cfg.head_dim;
+  const uint64_t page_rows = (uint64_t)h->cfg.n_kv_heads * (uint64_t)h->cfg.block_size;
+  nvattn_status st = encode_tensor_map_3d(
+      &e.map, base, D, page_rows, (uint64_t)h->cfg.n_layer * (uint64_t)h->cfg.num_blocks, D,
+      page_rows * D, (uint32_t)D, (uint32_t)box_rows, 1, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_DATA_TYPE_UINT8);
+  if (st != NVATTN_OK) return st;
+  keep_tensor_map(h, e);
   *out = e.map;
   return NVATTN_OK;
 }
@@ -215,6 +247,14 @@ nvattn_status nvattn_create(const nvattn_config* cfg, nvattn_handle** out) {
     else if (cudaMemset(h->decode_tickets, 0, tickets) != cudaSuccess)
       st = NVATTN_ERR_CUDA;
   }
+  if (st == NVATTN_OK) {
+    const size_t tickets = nvattn::part_ticket_count(h->sm_count) * sizeof(int);
+    if (cudaMalloc(&h->ws_part, nvattn::part_floats(h->sm_count) * sizeof(float)) != cudaSuccess ||
+        cudaMalloc(&h->part_tickets, tickets) != cudaSuccess)
+      st = NVATTN_ERR_NO_MEMORY;
+    else if (cudaMemset(h->part_tickets, 0, tickets) != cudaSuccess)
+      st = NVATTN_ERR_CUDA;
+  }
   if (st != NVATTN_OK) {
     cudaGetLastError();  // clear a sticky allocation error
     nvattn_destroy(h);
@@ -234,6 +274,8 @@ nvattn_status nvattn_destroy(nvattn_handle* h) {
   if (h->ws_ml) cudaFree(h->ws_ml);
   if (h->decode_tickets) cudaFree(h->decode_tickets);
   if (h->q_step) cudaFree(h->q_step);
+  if (h->ws_part) cudaFree(h->ws_part);
+  if (h->part_tickets) cudaFree(h->part_tickets);
   for (int p = 0; p < h->g_ranks; ++p)
     if (p != h->g_rank && h->g_peer[p] != nullptr) cudaIpcCloseMemHandle(h->g_peer[p]);
   if (h->g_own) cudaFree(h->g_own);
@@ -260,7 +302,9 @@ nvattn_status nvattn_get_error(nvattn_handle* h, int64_t* detail) {
   if (st.code == NVATTN_ERR_TIMEOUT &&
       (cudaMemset(h->decode_tickets, 0,
                   (size_t)h->cfg.max_seqs * h->cfg.n_kv_heads * sizeof(int)) != cudaSuccess ||
-       cudaMemset(h->prefill_sched_dev, 0, 2 * sizeof(int)) != cudaSuccess))
+       cudaMemset(h->prefill_sched_dev, 0, 2 * sizeof(int)) != cudaSuccess ||
+       cudaMemset(h->part_tickets, 0,
+                  nvattn::part_ticket_count(h->sm_count) * sizeof(int)) != cudaSuccess))
     return NVATTN_ERR_CUDA;
   // ...and ends the peer-memory gather: the ranks' step counters and this
   // rank's count of final-row CTAs no longer agree, so a later step could
@@ -715,6 +759,99 @@ nvattn_status nvattn_paged_prefill_rows(nvattn_handle* h, int layer, int n_seqs,
   return prefill_common(h, layer, n_seqs, n_tokens, q_dev, cu_q_lens_dev, q_starts_dev,
                         context_lens_dev, block_tables_dev, max_blocks, max_q_len, k_cache_dev,
                         v_cache_dev, k_rows_f16_dev, v_rows_f16_dev, out_dev, stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// 8-bit paged cache, token log-probabilities
+// ---------------------------------------------------------------------------
+namespace {
+
+// Payload and scales of an 8-bit K or V cache.
+bool q8_cache_ok(const uint8_t* q8, const float* scale) {
+  return q8 != nullptr && scale != nullptr && aligned16(q8) && aligned16(scale);
+}
+
+}  // namespace
+
+extern "C" {
+
+nvattn_status nvattn_kv_store_q8(nvattn_handle* h, int layer, int n_tokens, const float* q_dev,
+                                 const float* k_dev, const float* v_dev,
+                                 const uint16_t* q_norm_w_dev, const uint16_t* k_norm_w_dev,
+                                 const int32_t* positions_dev, const int32_t* slot_mapping_dev,
+                                 void* q_out_dev, nvattn_dtype q_out_dtype, uint8_t* k_q8_dev,
+                                 float* k_scale_dev, uint8_t* v_q8_dev, float* v_scale_dev,
+                                 uint16_t* k_rows_f16_dev, uint16_t* v_rows_f16_dev,
+                                 nvattn_stream_t stream) {
+  if (h == nullptr || layer < 0 || layer >= h->cfg.n_layer || n_tokens < 0)
+    return NVATTN_ERR_INVALID_ARG;
+  if (q_out_dtype != NVATTN_DTYPE_F32 && q_out_dtype != NVATTN_DTYPE_BF16 &&
+      q_out_dtype != NVATTN_DTYPE_F16)
+    return NVATTN_ERR_INVALID_ARG;
+  if (n_tokens == 0) return NVATTN_OK;
+  const void* ptrs[] = {q_dev, k_dev, v_dev, q_norm_w_dev, k_norm_w_dev, q_out_dev};
+  for (const void* p : ptrs)
+    if (p == nullptr || !aligned16(p)) return NVATTN_ERR_INVALID_ARG;
+  if (positions_dev == nullptr || slot_mapping_dev == nullptr ||
+      !q8_cache_ok(k_q8_dev, k_scale_dev) || !q8_cache_ok(v_q8_dev, v_scale_dev) ||
+      (k_rows_f16_dev == nullptr) != (v_rows_f16_dev == nullptr) || !aligned16(k_rows_f16_dev) ||
+      !aligned16(v_rows_f16_dev))
+    return NVATTN_ERR_INVALID_ARG;
+  DeviceGuard guard(h->cfg.device);
+  if (!guard.ok()) return NVATTN_ERR_CUDA;
+  return nvattn::launch_kv_store_q8(h, layer, n_tokens, q_dev, k_dev, v_dev, q_norm_w_dev,
+                                    k_norm_w_dev, positions_dev, slot_mapping_dev, q_out_dev,
+                                    q_out_dtype, k_q8_dev, k_scale_dev, v_q8_dev, v_scale_dev,
+                                    k_rows_f16_dev, v_rows_f16_dev,
+                                    reinterpret_cast<cudaStream_t>(stream));
+}
+
+nvattn_status nvattn_kv_load_q8(nvattn_handle* h, int layer, int n_tokens,
+                                const int32_t* slot_mapping_dev, const uint8_t* k_q8_dev,
+                                const float* k_scale_dev, const uint8_t* v_q8_dev,
+                                const float* v_scale_dev, nvattn_dtype out_dtype, void* k_out_dev,
+                                void* v_out_dev, nvattn_stream_t stream) {
+  if (h == nullptr || layer < 0 || layer >= h->cfg.n_layer || n_tokens < 0 ||
+      (out_dtype != NVATTN_DTYPE_F32 && out_dtype != NVATTN_DTYPE_BF16 &&
+       out_dtype != NVATTN_DTYPE_F16))
+    return NVATTN_ERR_INVALID_ARG;
+  if (n_tokens == 0) return NVATTN_OK;
+  if (slot_mapping_dev == nullptr || !q8_cache_ok(k_q8_dev, k_scale_dev) ||
+      !q8_cache_ok(v_q8_dev, v_scale_dev) || k_out_dev == nullptr || v_out_dev == nullptr ||
+      !aligned16(k_out_dev) || !aligned16(v_out_dev))
+    return NVATTN_ERR_INVALID_ARG;
+  DeviceGuard guard(h->cfg.device);
+  if (!guard.ok()) return NVATTN_ERR_CUDA;
+  return nvattn::launch_kv_load_q8(h, layer, n_tokens, slot_mapping_dev, k_q8_dev, k_scale_dev,
+                                   v_q8_dev, v_scale_dev, out_dtype, k_out_dev, v_out_dev,
+                                   reinterpret_cast<cudaStream_t>(stream));
+}
+
+nvattn_status nvattn_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, const void* q_dev,
+                                     nvattn_dtype dtype, const uint8_t* k_q8_dev,
+                                     const float* k_scale_dev, const uint8_t* v_q8_dev,
+                                     const float* v_scale_dev, const int32_t* block_tables_dev,
+                                     int max_blocks, const int32_t* context_lens_dev,
+                                     int max_context_len, void* out_dev, nvattn_stream_t stream) {
+  if (h == nullptr || layer < 0 || layer >= h->cfg.n_layer || n_seqs < 0 ||
+      n_seqs > h->cfg.max_seqs || max_blocks <= 0 || max_context_len < 0 ||
+      max_context_len > h->cfg.max_context ||
+      (long long)max_context_len > (long long)max_blocks * h->cfg.block_size ||
+      (dtype != NVATTN_DTYPE_F32 && dtype != NVATTN_DTYPE_BF16))
+    return NVATTN_ERR_INVALID_ARG;
+  if (n_seqs == 0) return NVATTN_OK;
+  if (q_dev == nullptr || out_dev == nullptr || !aligned16(q_dev) || !aligned16(out_dev) ||
+      !q8_cache_ok(k_q8_dev, k_scale_dev) || !q8_cache_ok(v_q8_dev, v_scale_dev) ||
+      block_tables_dev == nullptr || context_lens_dev == nullptr)
+    return NVATTN_ERR_INVALID_ARG;
+  DeviceGuard guard(h->cfg.device);
+  if (!guard.ok()) return NVATTN_ERR_CUDA;
+  return nvattn::launch_paged_decode_q8(h, layer, n_seqs, q_dev, dtype, k_q8_dev, k_scale_dev,
+                                        v_q8_dev, v_scale_dev, block_tables_dev, max_blocks,
+                                        context_lens_dev, max_context_len, out_dev,
+                                        reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -255,6 +255,24 @@ __device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
   return r;
 }
 
+// Two e4m3 values (bits 0-15) -> f16x2, exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  return r;
+}
+
+// Four e4m3 values (byte 0 first) -> f32, exact.
+__device__ __forceinline__ void e4m3x4_to_f32(uint32_t w, float (&f)[4]) {
+  const uint32_t h[2] = {e4m3x2_to_f16x2(w & 0xffffu), e4m3x2_to_f16x2(w >> 16)};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+        : "=f"(f[2 * i]), "=f"(f[2 * i + 1])
+        : "r"(h[i]));
+}
+
 // True in one lane of a converged warp (elect.sync over all 32 lanes).  A
 // warp that runs an MMA-issuing loop converged keeps its descriptor and loop
 // values warp-uniform and elects the issuing lane only at each tcgen05

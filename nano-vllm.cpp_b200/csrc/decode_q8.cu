@@ -1,0 +1,540 @@
+// decode_q8.cu -- paged GQA decode attention over the 8-bit KV cache.
+//
+//   o = sum_t softmax_t(scale * s_k[t] * q.K8[t]) * s_v[t] * V8[t]
+//
+// K8, V8: e4m3 rows of 128, s_k, s_v: their power-of-two scales; pages
+// [layer][block][kv head][token][128], so a (block, kv head) is one contiguous
+// run of both.  Both scales leave the matrix products: s_k multiplies the
+// score, and s_v joins the exponent,
+//   x_t = scale * log2(e) * s_k[t] * (q.K8[t]) + log2 s_v[t]
+//   w_t = 2^(x_t - M),  o = sum w_t V8[t] / sum w_t / s_v[t],  M >= x_t - 8
+// so that the weights handed to the tensor cores are at most 2^8 times the
+// row's reference whatever the rows' scales are.
+//
+// Bound by memory: 264 bytes per cached token and kv head against 2 * 128 * 2
+// products per query head.  The rows of one kv head are at most eight, so the
+// products run as mma.sync m16n8k16 on f16 (which holds e4m3 exactly) with the
+// query rows in rows 0-7 and their f16 remainders in rows 8-15: queries and
+// weights carry 22 bits at no extra cost, which a 128-row tcgen05 tile could
+// not use, and the 8-bit rows go from shared memory through registers without
+// the widened copy in shared memory that a tcgen05 operand would need.
+//
+// Each warp works alone: 32-token steps, K and V tiles of 4 KiB each by TMA
+// (128-byte swizzle) and their scales by bulk copies into its own ring of
+// kStages, its own running reference M, sum and output.  A CTA's kWarps warps
+// take consecutive 32-token steps of a 128-token tile; the CTAs' tiles are
+// split evenly (tile_split.cuh).  At a unit's end the warps' results are
+// merged in shared memory, and where CTAs share a unit the last of them to
+// finish merges their partials in CTA order (the same sums on every run).
+//
+// Which lane reads what.  Within the eight tokens of a score tile, column n of
+// the product is token (n >> 1) | (n & 1) << 2, and of the 16-byte chunks of a
+// V row lane g takes chunk (g >> 1) | (g & 1) << 2: with the swizzle that
+// makes every 16-byte shared load of a quarter warp hit 32 distinct banks.  A
+// lane's 16 bytes of K feed four products (the dimension order inside a dot
+// product is free, and the query operand uses the same order); of V, 16
+// products of one dimension each, after pairing the bytes of two tokens.
+#include <atomic>
+
+#include "common.cuh"
+#include "internal.h"
+#include "tile_split.cuh"
+
+namespace nvattn {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kWarps = kQ8Warps;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStep = 32;                // tokens per warp step
+constexpr int kTile = kWarps * kStep;    // tokens per CTA tile
+constexpr int kStages = 2;
+constexpr int kRows = 8;                 // query rows per unit (GQA group, padded)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.0f;           // log2: rescale only past 2^8
+static_assert(kTile == 128, "a tile must not cross a block (block sizes are multiples of 128)");
+
+struct Q8Params {
+  int Hq, Hkv, G, layer, block_size, max_blocks, n_seqs, max_context;
+  long long num_blocks;
+  float scale_log2;
+  const void* q;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  void* out;
+  float* part;   // [CTA][2][kQ8PartFloats]
+  int* tickets;  // [CTA], zero between launches
+  DeviceStatus* status;
+};
+
+struct __align__(1024) WarpRing {
+  uint8_t k[kStages][kStep * kD];
+  uint8_t v[kStages][kStep * kD];
+};
+
+struct __align__(1024) Q8Smem {
+  WarpRing ring[kWarps];
+  float ks[kWarps][kStages][kStep];
+  float vs[kWarps][kStages][kStep];
+  float4 tok[kWarps][kStep];  // {score factor, log2 s_v, 1 / s_v, 0} of the step's tokens
+  float o[kWarps][kRows][kD];
+  float m[kWarps][kRows], l[kWarps][kRows];
+  uint64_t full[kWarps][kStages];
+  int abort_flag;
+  int last;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// hi = f16(x), lo = f16(x - hi) of two values, packed.
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = cvt_f16x2(x0, x1);
+  float h0, h1;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(h0), "=f"(h1)
+      : "r"(hi));
+  lo = cvt_f16x2(x0 - h0, x1 - h1);
+}
+
+// Where a walk over the CTA's run of tiles stands.
+struct Walk {
+  long long at;  // global tile index
+  int seq, head, tile, ctx, n_tiles;
+};
+
+__device__ __forceinline__ int clamped_ctx(const Q8Params& p, int seq) {
+  return min(max(p.context_lens[seq], 0), p.max_context);
+}
+__device__ __forceinline__ int tiles_of(int ctx) { return max(1, (ctx + kTile - 1) / kTile); }
+
+__device__ __forceinline__ void walk_next(const Q8Params& p, long long end, Walk& w) {
+  ++w.at;
+  if (++w.tile < w.n_tiles) return;
+  w.tile = 0;
+  if (++w.head < p.Hkv) return;
+  w.head = 0;
+  ++w.seq;
+  if (w.at < end) {
+    w.ctx = clamped_ctx(p, w.seq);
+    w.n_tiles = tiles_of(w.ctx);
+  }
+}
+
+// The query rows of (seq, head) as mma operands: rows scaled by a power of
+// two so that max|q| lies in [1, 2), hi parts in rows 0-7, remainders in 8-15.
+// Returns the factor that undoes the scaling (of row g).
+template <bool kBf16>
+__device__ __forceinline__ float load_q(const Q8Params& p, int seq, int head, int g, int c,
+                                        uint32_t (&a)[8][4]) {
+  float x[2][16];
+  const bool real = g < p.G;
+  const long long off = ((long long)seq * p.Hq + (long long)head * p.G + g) * kD + 16 * c;
+  uint32_t big = 0;
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[hf][i] = 0.0f;
+    if (real) {
+      if constexpr (kBf16) {
+        const uint4* src =
+            reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + off + 64 * hf);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = src[i];
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[hf][8 * i + 2 * e] = bf16lo_to_f32(u[e]);
+            x[hf][8 * i + 2 * e + 1] = bf16hi_to_f32(u[e]);
+          }
+        }
+      } else {
+        const float4* src =
+            reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + off + 64 * hf);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 v = src[i];
+          x[hf][4 * i] = v.x; x[hf][4 * i + 1] = v.y; x[hf][4 * i + 2] = v.z; x[hf][4 * i + 3] = v.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) big = max(big, __float_as_uint(x[hf][i]) & 0x7fffffffu);
+  }
+  big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+  big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+  int e = (int)(big >> 23) - 127;
+  e = (big == 0 || big >= 0x7f800000u) ? 0 : min(max(e, -100), 100);
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t* f = a[4 * hf + i];
+      split_f16(x[hf][4 * i] * down, x[hf][4 * i + 1] * down, f[0], f[1]);
+      split_f16(x[hf][4 * i + 2] * down, x[hf][4 * i + 3] * down, f[2], f[3]);
+    }
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void write_out(const Q8Params& p, int seq, int head, int row, int d,
+                                          float o, float l) {
+  const float y = l == 0.0f ? 0.0f : o / l;  // no key: zeros
+  const long long i = ((long long)seq * p.Hq + (long long)head * p.G + row) * kD + d;
+  if constexpr (kBf16)
+    static_cast<uint16_t*>(p.out)[i] = (uint16_t)f32_to_bf16_bits(y);
+  else
+    static_cast<float*>(p.out)[i] = y;
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads, 2)
+    decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, Q8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  Q8Smem& sm = *reinterpret_cast<Q8Smem*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&sm.full[warp][i], 1);
+    fence_barrier_init();
+  }
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    sm.last = timeout_recorded(p.status);  // then: skip the work
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  volatile int* abort_flag = &sm.abort_flag;
+  const tilesplit::Run run =
+      tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, [&](int s) {
+        return tilesplit::SeqTiles{p.Hkv, tiles_of(clamped_ctx(p, s))};
+      });
+  __syncthreads();
+  if (run.begin >= run.end || sm.last) return;
+
+  Walk w;
+  w.at = run.begin;
+  w.seq = run.seq;
+  w.ctx = clamped_ctx(p, w.seq);
+  w.n_tiles = tiles_of(w.ctx);
+  w.head = (int)((run.begin - run.seq_first) / w.n_tiles);
+  w.tile = (int)((run.begin - run.seq_first) % w.n_tiles);
+
+  // ---- loads: one step = this warp's 32 tokens of a tile ----
+  Walk ahead = w;
+  int issued = 0, used = 0;
+  const uint64_t policy = l2_policy_evict_first();
+  auto block_of = [&](const Walk& x) -> int {
+    const int t0 = x.tile * kTile + warp * kStep;
+    if (x.at >= run.end || t0 >= x.ctx) return 0;
+    return p.block_tables[(long long)x.seq * p.max_blocks + t0 / p.block_size];
+  };
+  int next_bid = block_of(ahead);
+  auto issue = [&]() {  // the step at `ahead`, if it has tokens; moves `ahead` on
+    const int t0 = ahead.tile * kTile + warp * kStep;
+    const bool some = t0 < ahead.ctx;
+    long long bid = next_bid;
+    const int head = ahead.head;
+    const int seq = ahead.seq, raw = ahead.tile == 0 && ahead.head == 0;
+    walk_next(p, run.end, ahead);
+    next_bid = block_of(ahead);  // used a step later: its latency is off the path
+    if (raw && warp == 0 && lane == 0) {
+      const int ctx = p.context_lens[seq];
+      if (ctx < 0 || ctx > p.max_context)
+        record_error(p.status, NVATTN_ERR_OUT_OF_RANGE, 91, ctx);
+    }
+    if (!some) return;
+    if (lane == 0) {
+      if (bid < 0 || bid >= p.num_blocks) {
+        record_error(p.status, NVATTN_ERR_OUT_OF_RANGE, 92, bid);
+        bid = 0;  // keep the ring in step; the result is flagged
+      }
+      const int st = issued % kStages;
+      uint64_t* bar = &sm.full[warp][st];
+      const int page = (int)((long long)p.layer * p.num_blocks + bid);
+      const int row = head * p.block_size + t0 % p.block_size;
+      const long long srow = (long long)page * p.Hkv * p.block_size + row;
+      mbar_arrive_expect_tx(bar, 2 * kStep * (kD + 4));
+      tma_load_3d_hint(sm.ring[warp].k[st], &tm_k, bar, 0, row, page, policy);
+      tma_load_3d_hint(sm.ring[warp].v[st], &tm_v, bar, 0, row, page, policy);
+      bulk_load(sm.ks[warp][st], p.k_scale + srow, kStep * 4, bar, policy);
+      bulk_load(sm.vs[warp][st], p.v_scale + srow, kStep * 4, bar, policy);
+    }
+    ++issued;
+  };
+  // (`ahead` may run past the last tile by the ring's depth: no step there)
+  for (int i = 0; i < kStages && ahead.at < run.end; ++i) issue();
+
+  uint32_t qa[8][4];
+  float o[16][4];
+  const int pr = (g >> 1) | ((g & 1) << 2);
+
+  while (w.at < run.end) {
+    // ---- one unit's part of the run ----
+    const int seq = w.seq, head = w.head, first = w.tile, n_tiles = w.n_tiles, ctx = w.ctx;
+    const long long unit0 = w.at - w.tile;
+    const float up = load_q<kBf16>(p, seq, head, g, c, qa);
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+
+    int done = 0;  // tiles of the unit in this run
+    do {
+      const int t0 = w.tile * kTile + warp * kStep;
+      if (t0 < ctx) {
+        const int st = used % kStages;
+        mbar_wait(&sm.full[warp][st], (used / kStages) & 1, p.status, abort_flag, 93);
+        ++used;
+        uint8_t* kt = sm.ring[warp].k[st];
+        uint8_t* vt = sm.ring[warp].v[st];
+        const int n = min(ctx - t0, kStep);
+        // ---- the tokens' factors ----
+        {
+          const float sk = sm.ks[warp][st][lane], sv = sm.vs[warp][st][lane];
+          const uint32_t b = __float_as_uint(sv);
+          // a NaN scale (a row that held a NaN or an infinity) stays NaN
+          float4 f = make_float4(sk * p.scale_log2, (float)((int)(b >> 23) - 127) + (sv - sv),
+                                 __uint_as_float((254u << 23) - (b & 0x7f800000u)), 0.0f);
+          if (lane >= n) {
+            // Slots behind the context hold anything: weight zero, and rows
+            // of zeros so that no NaN meets it.
+            f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              reinterpret_cast<uint4*>(kt + lane * kD)[i] = z;
+              reinterpret_cast<uint4*>(vt + lane * kD)[i] = z;
+            }
+          }
+          if (n < kStep) fence_proxy_async_smem();  // before the ring's next copy into this stage
+          sm.tok[warp][lane] = f;
+          __syncwarp();
+        }
+        // ---- scores: 4 tiles of 8 tokens ----
+        float x[4][2], inv[4][2];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint8_t* row = kt + (8 * nt + pr) * kD;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint4 v = *reinterpret_cast<const uint4*>(row + (((c + 4 * hf) ^ pr) << 4));
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma_f16(s, qa[4 * hf + i], e4m3x2_to_f16x2(u[i] & 0xffffu),
+                      e4m3x2_to_f16x2(u[i] >> 16));
+          }
+          const float4 f0 = sm.tok[warp][8 * nt + c], f1 = sm.tok[warp][8 * nt + c + 4];
+          x[nt][0] = fmaf((s[0] + s[2]) * up, f0.x, f0.y);
+          x[nt][1] = fmaf((s[1] + s[3]) * up, f1.x, f1.y);
+          inv[nt][0] = f0.z;
+          inv[nt][1] = f1.z;
+        }
+        float mx = fmax3(fmax3(x[0][0], x[0][1], x[1][0]), fmax3(x[1][1], x[2][0], x[2][1]),
+                         fmaxf(x[3][0], x[3][1]));
+        if (__any_sync(0xffffffffu, mx > m + kSlack)) {
+          // (rare after the first step: the reference moves in strides of 2^8)
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = mx > m + kSlack ? mx : m;
+          const float alpha = m_new == m ? 1.0f : fast_exp2(m - m_new);
+          m = m_new;
+          l *= alpha;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] *= alpha;
+        }
+        uint32_t wa[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          // x = -inf gives 0 unless no key has been seen (m = -inf too)
+          const float w0 = x[nt][0] == -INFINITY ? 0.0f : fast_exp2(x[nt][0] - m);
+          const float w1 = x[nt][1] == -INFINITY ? 0.0f : fast_exp2(x[nt][1] - m);
+          l = fmaf(w0, inv[nt][0], l);
+          l = fmaf(w1, inv[nt][1], l);
+          split_f16(w0, w1, wa[nt >> 1][2 * (nt & 1)], wa[nt >> 1][2 * (nt & 1) + 1]);
+        }
+        // ---- o += w V8 ----
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          uint32_t v[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 16 * ks + c + 4 * i;
+            const uint4 t = *reinterpret_cast<const uint4*>(vt + r * kD + ((pr ^ (r & 7)) << 4));
+            v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a01 = __byte_perm(v[0][i], v[1][i], 0x5140);
+            const uint32_t a23 = __byte_perm(v[0][i], v[1][i], 0x7362);
+            const uint32_t b01 = __byte_perm(v[2][i], v[3][i], 0x5140);
+            const uint32_t b23 = __byte_perm(v[2][i], v[3][i], 0x7362);
+            mma_f16(o[4 * i], wa[ks], e4m3x2_to_f16x2(a01 & 0xffffu), e4m3x2_to_f16x2(b01 & 0xffffu));
+            mma_f16(o[4 * i + 1], wa[ks], e4m3x2_to_f16x2(a01 >> 16), e4m3x2_to_f16x2(b01 >> 16));
+            mma_f16(o[4 * i + 2], wa[ks], e4m3x2_to_f16x2(a23 & 0xffffu), e4m3x2_to_f16x2(b23 & 0xffffu));
+            mma_f16(o[4 * i + 3], wa[ks], e4m3x2_to_f16x2(a23 >> 16), e4m3x2_to_f16x2(b23 >> 16));
+          }
+        }
+        __syncwarp();  // every lane has read the stage
+      }
+      if (ahead.at < run.end) issue();
+      walk_next(p, run.end, w);
+      ++done;
+    } while (w.at < run.end && w.tile != 0);
+
+    // ---- merge the warps (thread = dimension) ----
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (c == 0) {
+      sm.m[warp][g] = m;
+      sm.l[warp][g] = l;
+    }
+    if (g < p.G) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float4 a, b;
+        a = make_float4(o[4 * j][0] + o[4 * j][2], o[4 * j + 1][0] + o[4 * j + 1][2],
+                        o[4 * j + 2][0] + o[4 * j + 2][2], o[4 * j + 3][0] + o[4 * j + 3][2]);
+        b = make_float4(o[4 * j][1] + o[4 * j][3], o[4 * j + 1][1] + o[4 * j + 1][3],
+                        o[4 * j + 2][1] + o[4 * j + 2][3], o[4 * j + 3][1] + o[4 * j + 3][3]);
+        *reinterpret_cast<float4*>(&sm.o[warp][g][16 * c + 4 * j]) = a;
+        *reinterpret_cast<float4*>(&sm.o[warp][g][64 + 16 * c + 4 * j]) = b;
+      }
+    }
+    __syncthreads();
+    const bool whole = first == 0 && done == n_tiles;
+    const int d = threadIdx.x;
+    float* part = p.part + ((long long)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * kQ8PartFloats;
+    for (int r = 0; r < p.G; ++r) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.m[i][r]);
+      float O = 0.0f, L = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const float f = sm.m[i][r] == -INFINITY ? 1.0f : fast_exp2(sm.m[i][r] - M);
+        O = fmaf(sm.o[i][r][d], f, O);
+        L = fmaf(sm.l[i][r], f, L);
+      }
+      if (whole) {
+        write_out<kBf16>(p, seq, head, r, d, O, L);
+      } else {
+        part[r * kD + d] = O;
+        if (d == 0) {
+          part[kRows * kD + r] = M;
+          part[kRows * kD + kRows + r] = L;
+        }
+      }
+    }
+    if (!whole) {
+      const int c0 = (int)(unit0 / run.per), c1 = (int)((unit0 + n_tiles - 1) / run.per);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+        if (last) atomicExch(p.tickets + c0, 0);  // re-armed for the next launch
+        sm.last = last;
+      }
+      __syncthreads();
+      if (sm.last) {
+        __threadfence();
+        for (int r = 0; r < p.G; ++r) {
+          float M = -INFINITY;
+          for (int i = c0; i <= c1; ++i)
+            M = fmaxf(M, __ldcg(p.part + ((long long)i * 2 + (i == c0)) * kQ8PartFloats +
+                                kRows * kD + r));
+          float O = 0.0f, L = 0.0f;
+          for (int i = c0; i <= c1; ++i) {
+            const float* q = p.part + ((long long)i * 2 + (i == c0)) * kQ8PartFloats;
+            const float mi = __ldcg(q + kRows * kD + r);
+            const float f = mi == -INFINITY ? 1.0f : fast_exp2(mi - M);
+            O = fmaf(__ldcg(q + r * kD + d), f, O);
+            L = fmaf(__ldcg(q + kRows * kD + kRows + r), f, L);
+          }
+          write_out<kBf16>(p, seq, head, r, d, O, L);
+        }
+      }
+    }
+    __syncthreads();  // the merge buffers are free
+  }
+  // After a wait that ran out, copies may still be in flight: wait (bounded)
+  // for the ring's last ones before the CTA's shared memory goes away.
+  if (*abort_flag && lane == 0)
+    for (int i = max(0, issued - kStages); i < issued; ++i)
+      mbar_wait(&sm.full[warp][i % kStages], (i / kStages) & 1, p.status, 94);
+}
+
+}  // namespace
+
+nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, const void* q,
+                                     nvattn_dtype dtype, const uint8_t* k_q8,
+                                     const float* k_scale, const uint8_t* v_q8,
+                                     const float* v_scale, const int32_t* block_tables,
+                                     int max_blocks, const int32_t* context_lens,
+                                     int max_context_len, void* out, cudaStream_t stream) {
+  if (n_seqs == 0) return NVATTN_OK;
+  CUtensorMap tk, tv;
+  nvattn_status st = get_q8_tensor_map(h, k_q8, kStep, &tk);
+  if (st != NVATTN_OK) return st;
+  st = get_q8_tensor_map(h, v_q8, kStep, &tv);
+  if (st != NVATTN_OK) return st;
+  Q8Params p = {};
+  p.Hq = h->cfg.n_q_heads;
+  p.Hkv = h->cfg.n_kv_heads;
+  p.G = p.Hq / p.Hkv;
+  p.layer = layer;
+  p.block_size = h->cfg.block_size;
+  p.max_blocks = max_blocks;
+  p.n_seqs = n_seqs;
+  p.max_context = max_context_len;
+  p.num_blocks = h->cfg.num_blocks;
+  p.scale_log2 = h->cfg.scale * kLog2e;
+  p.q = q;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.block_tables = block_tables;
+  p.context_lens = context_lens;
+  p.out = out;
+  p.part = h->ws_part;
+  p.tickets = h->part_tickets;
+  p.status = h->status_dev;
+  const size_t smem = sizeof(Q8Smem) + 1024;
+  static_assert(sizeof(Q8Smem) + 1024 <= 113 * 1024, "two CTAs per SM");
+  // (atomic: handles on different threads may launch at the same time)
+  static std::atomic<unsigned long long> attr_set_mask{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return NVATTN_ERR_CUDA;
+  if (dev >= 64 || !(attr_set_mask.load(std::memory_order_relaxed) & (1ull << dev))) {
+    if (cudaFuncSetAttribute(decode_q8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem) != cudaSuccess ||
+        cudaFuncSetAttribute(decode_q8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem) != cudaSuccess)
+      return NVATTN_ERR_CUDA;
+    if (dev < 64) attr_set_mask.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  const int grid = kQ8CtasPerSm * h->sm_count;
+  if (dtype == NVATTN_DTYPE_BF16)
+    decode_q8_kernel<true><<<grid, kThreads, smem, stream>>>(tk, tv, p);
+  else
+    decode_q8_kernel<false><<<grid, kThreads, smem, stream>>>(tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? NVATTN_OK : NVATTN_ERR_CUDA;
+}
+
+}  // namespace nvattn

@@ -23,6 +23,7 @@ struct NvattnTensorMapEntry {
   int box_d;     // inner box extent (elements)
   int box_rows;  // tokens per box
   int swizzle;   // CUtensorMapSwizzle value
+  bool q8;       // 8-bit pages (get_q8_tensor_map) instead of a bf16 cache
   CUtensorMap map;
 };
 
@@ -45,6 +46,12 @@ struct nvattn_handle {
   // the normed, rotated q of a decode step run as two launches (the KV store
   // writes it, the decode reads it): [max_seqs][n_q_heads][head_dim] f32
   float* q_step = nullptr;
+
+  // Partial results of the attention kernels that split the batch's key tiles
+  // evenly over their CTAs (tile_split.cuh): two per CTA, and one ticket per
+  // CTA, zero between launches.
+  float* ws_part = nullptr;
+  int* part_tickets = nullptr;
 
   // all-gather of decode outputs over peer memory (nvattn_gather_*): this
   // rank's allocation holds [2 step parities][g_ranks][g_slice] f32 and, at
@@ -92,6 +99,12 @@ constexpr int kMaxDecodeSeqs = 65535;
 nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d,
                                    int box_rows, int swizzle, CUtensorMap* out);
 
+// Copies into *out a TMA descriptor over the K or V pages of an 8-bit cache
+// (all layers): bytes, dims {128, n_kv_heads * block_size, n_layer *
+// num_blocks}, box {128, box_rows, 1}, 128-byte swizzle; cached as above.
+nvattn_status get_q8_tensor_map(nvattn_handle* h, const void* base, int box_rows,
+                                CUtensorMap* out);
+
 // Generic 3-D tensor map of 16-bit elements (bf16 caches; f16 Q in prefill).
 nvattn_status encode_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t d0,
                                    uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
@@ -105,6 +118,34 @@ nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const f
                               const int32_t* slots, void* q_out, nvattn_dtype q_out_dtype,
                               uint16_t* k_cache, uint16_t* v_cache, uint16_t* k_rows,
                               uint16_t* v_rows, cudaStream_t stream);
+
+// The 8-bit paged cache: the store (kv_store.cu), the read-back (kv_q8.cu)
+// and the decode over it (decode_q8.cu).
+nvattn_status launch_kv_store_q8(nvattn_handle* h, int layer, int n_tokens, const float* q,
+                                 const float* k, const float* v, const uint16_t* qw,
+                                 const uint16_t* kw, const int32_t* positions,
+                                 const int32_t* slots, void* q_out, nvattn_dtype q_out_dtype,
+                                 uint8_t* k_q8, float* k_scale, uint8_t* v_q8, float* v_scale,
+                                 uint16_t* k_rows, uint16_t* v_rows, cudaStream_t stream);
+nvattn_status launch_kv_load_q8(nvattn_handle* h, int layer, int n_tokens, const int32_t* slots,
+                                const uint8_t* k_q8, const float* k_scale, const uint8_t* v_q8,
+                                const float* v_scale, nvattn_dtype out_dtype, void* k_out,
+                                void* v_out, cudaStream_t stream);
+constexpr int kQ8Warps = 4;
+constexpr int kQ8CtasPerSm = 2;
+// one partial: 8 rows of 128, then 8 references and 8 sums
+constexpr int kQ8PartFloats = 8 * 128 + 16;
+// The workspace of the evenly split kernels (ws_part, part_tickets).
+inline size_t part_ticket_count(int sm_count) { return (size_t)kQ8CtasPerSm * sm_count; }
+inline size_t part_floats(int sm_count) {
+  return 2 * part_ticket_count(sm_count) * kQ8PartFloats;
+}
+nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, const void* q,
+                                     nvattn_dtype dtype, const uint8_t* k_q8,
+                                     const float* k_scale, const uint8_t* v_q8,
+                                     const float* v_scale, const int32_t* block_tables,
+                                     int max_blocks, const int32_t* context_lens,
+                                     int max_context_len, void* out, cudaStream_t stream);
 
 nvattn_status launch_paged_decode(nvattn_handle* h, int layer, int n_seqs, const float* q,
                                   const uint16_t* k_cache, const uint16_t* v_cache,

@@ -83,15 +83,73 @@ struct KvStoreParams {
   uint16_t* v_cache;
   uint16_t* k_rows;  // nullable: f16 copies of the stored K rows, [n_tokens][Hkv][128]
   uint16_t* v_rows;  // nullable: f16 copies of the V rows
+  // 8-bit cache (kQ8 kernels; k_cache / v_cache then unused): e4m3 pages
+  // [layer][block][Hkv][block_size][128] and one scale per row
+  int block_size;
+  long long num_blocks;
+  uint8_t* k_q8;
+  uint8_t* v_q8;
+  float* k_scale;
+  float* v_scale;
   DeviceStatus* status;
 };
 
 // q_out element types (template argument of the row kernels).
 constexpr int kQOutF32 = 0, kQOutBf16 = 1, kQOutF16 = 2;
 
+// Four floats -> e4m3, round to nearest even; |y| <= 448, so nothing
+// saturates.
+__device__ __forceinline__ uint32_t pack4_e4m3(const float* y) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]));
+  return r;
+}
+
+// Writes one row of the 8-bit cache: a = max|x| over the group's eight lanes,
+// the scale 2^E with the smallest E such that a <= 448 * 2^E, and the 128
+// values e4m3(x / 2^E).  A power of two costs e4m3 no precision (it is a
+// floating format) and makes x / 2^E and the value read back exact, so the
+// one rounding of a stored value is e4m3's own, 2^-4 relative.  E >= -100
+// keeps the scale, its reciprocal and their products far inside f32 and bf16;
+// an all-zero row takes scale 1.  e4m3 has no infinity: a row that holds a
+// NaN or an infinity stores zeros under a NaN scale, so all of it reads back
+// as NaN.
+__device__ __forceinline__ void store_row_q8(const KvStoreParams& p, const float (&x)[2 * kPer],
+                                             int kind, int head, int slot, int l8) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int e = 0; e < 2 * kPer; ++e) a = max(a, __float_as_uint(x[e]) & 0x7fffffffu);
+  const uint32_t group = 0xffu << (threadIdx.x & 24);  // the row's lanes branch together
+#pragma unroll
+  for (int o = kLanesPerRow / 2; o >= 1; o >>= 1) a = max(a, __shfl_xor_sync(group, a, o));
+  // a = 1.m * 2^(field - 127) against 448 = 1.75 * 2^8
+  const int E = max((int)(a >> 23) - 127 - ((a & 0x7fffffu) <= 0x600000u ? 8 : 7), -100);
+  const bool finite = a < 0x7f800000u;
+  const bool plain = finite && a != 0;
+  const float scale = plain    ? __uint_as_float((uint32_t)(E + 127) << 23)
+                      : finite ? 1.0f
+                               : __uint_as_float(0x7fc00000u);
+  const float inv = plain ? __uint_as_float((uint32_t)(127 - E) << 23) : 0.0f;
+  float y[2 * kPer];
+#pragma unroll
+  for (int e = 0; e < 2 * kPer; ++e) y[e] = finite ? x[e] * inv : 0.0f;
+  const long long row = (((long long)p.layer * p.num_blocks + slot / p.block_size) * p.Hkv + head) *
+                            p.block_size + slot % p.block_size;
+  uint8_t* dst = (kind == 1 ? p.k_q8 : p.v_q8) + row * kD + kPer * l8;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack4_e4m3(y), pack4_e4m3(y + 4));
+  *reinterpret_cast<uint2*>(dst + kHalf) =
+      make_uint2(pack4_e4m3(y + kPer), pack4_e4m3(y + kPer + 4));
+  if (l8 == 0) (kind == 1 ? p.k_scale : p.v_scale)[row] = scale;
+}
+
 // Writes the finished row: q rows to q_out, k/v rows to slot_mapping[t] of
 // the cache (slot < 0: not stored; slot >= n_slots: reported).
-template <int kQOut>
+template <int kQOut, bool kQ8>
 __device__ __forceinline__ void store_row(const KvStoreParams& p, const float (&x)[2 * kPer],
                                           int t, int rr, int kind, int slot, bool nan_rule,
                                           int l8) {
@@ -130,6 +188,10 @@ __device__ __forceinline__ void store_row(const KvStoreParams& p, const float (&
     record_error(p.status, NVATTN_ERR_OUT_OF_RANGE, 2, slot);
     return;
   }
+  if constexpr (kQ8) {
+    store_row_q8(p, x, kind, head, slot, l8);
+    return;
+  }
   uint16_t* dst = (kind == 1 ? p.k_cache : p.v_cache) +
                   (((long long)p.layer * p.n_slots + slot) * p.Hkv + head) * kD + kPer * l8;
   *reinterpret_cast<uint4*>(dst) = pack8_bf16(x, nan_rule);
@@ -140,7 +202,7 @@ __device__ __forceinline__ void store_row(const KvStoreParams& p, const float (&
 // calls this, `active` false for padding rows).  get_w(w) and get_cs(c, sn)
 // supply the lane's norm weights and cos/sin values; they run after the
 // norm's dependency chain so the values are live only where they are used.
-template <int kQOut, class GetW, class GetCs>
+template <int kQOut, bool kQ8, class GetW, class GetCs>
 __device__ __forceinline__ void finish_row(const KvStoreParams& p, float (&x)[2 * kPer],
                                            bool active, int t, int rr, int kind, int pos,
                                            bool pos_ok, int slot, GetW get_w, bool w_tame,
@@ -160,7 +222,7 @@ __device__ __forceinline__ void finish_row(const KvStoreParams& p, float (&x)[2 
     norm_rope(x, scale, w, c, sn);
     nan_rule = nan_rule || !w_tame;
   }
-  store_row<kQOut>(p, x, t, rr, kind, slot, nan_rule, l8);
+  store_row<kQOut, kQ8>(p, x, t, rr, kind, slot, nan_rule, l8);
 }
 
 // Input row of flattened row (t, rr): q, k or v head row.
@@ -173,7 +235,7 @@ __device__ __forceinline__ const float* row_src(const KvStoreParams& p, int t, i
 // kOneRow: every group stores one row (rows_per_group == 1), so nothing is
 // prefetched and three blocks fit on an SM; otherwise the group prefetches
 // its next row while it finishes the current one, two blocks per SM.
-template <int kQOut, bool kOneRow>
+template <int kQOut, bool kOneRow, bool kQ8>
 __global__ void __launch_bounds__(kThreads, kOneRow ? 3 : 2) kv_store_rows_kernel(KvStoreParams p) {
   const int l8 = threadIdx.x & 7;  // lane within the row's 8-lane group
   const int rows_per_token = p.Hq + 2 * p.Hkv;
@@ -226,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, kOneRow ? 3 : 2) kv_store_rows_kerne
       load_weights(kind == 0 ? p.qw : p.kw, l8, lw);
     }
     const int slot = (valid && kind != 0) ? p.slots[t_row] : 0;
-    finish_row<kQOut>(p, x, valid, t_row, rr_row, kind, pos, pos_ok, slot,
+    finish_row<kQOut, kQ8>(p, x, valid, t_row, rr_row, kind, pos, pos_ok, slot,
                           [&](float (&w)[2 * kPer]) {
 #pragma unroll
                             for (int e = 0; e < kPer; ++e) {
@@ -283,7 +345,7 @@ __device__ __forceinline__ int lane_weight_slot(int el) {
 // The header holds the ring's barriers and, per stage, the chunk's positions
 // and slots (written by the producer warp before it arms the stage, so the
 // consumers never wait on a global load).
-template <int kQOut>
+template <int kQOut, bool kQ8>
 __global__ void __launch_bounds__(kStageMaxThreads, 1)
     kv_store_staged_kernel(KvStoreParams p, StagedPlan plan) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -426,7 +488,7 @@ __global__ void __launch_bounds__(kStageMaxThreads, 1)
       const bool pos_ok = pos >= 0 && pos < p.max_position;
       const float4* cs4 = reinterpret_cast<const float4*>(st + (stage_rows + g.tl) * kRowBytes);
       const float4* w4 = reinterpret_cast<const float4*>(wsm + (g.kind == 0 ? 0 : kD)) + l8;
-      finish_row<kQOut>(
+      finish_row<kQOut, kQ8>(
           p, x, active, t0 + g.tl, g.rr, g.kind, pos, pos_ok, mslot[g.tl],
           [&](float (&w)[2 * kPer]) {
 #pragma unroll
@@ -479,7 +541,7 @@ StagedPlan plan_staged(int n_tokens, int Hq, int Hkv) {
   return s;
 }
 
-template <int kQOut>
+template <int kQOut, bool kQ8>
 nvattn_status launch_staged(const KvStoreParams& p, const StagedPlan& plan, int sm_count,
                             cudaStream_t stream) {
   // (atomic: handles on different threads may launch at the same time)
@@ -487,7 +549,7 @@ nvattn_status launch_staged(const KvStoreParams& p, const StagedPlan& plan, int 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NVATTN_ERR_CUDA;
   if (dev >= 64 || !(attr_set_mask.load(std::memory_order_relaxed) & (1ull << dev))) {
-    if (cudaFuncSetAttribute(kv_store_staged_kernel<kQOut>,
+    if (cudaFuncSetAttribute(kv_store_staged_kernel<kQOut, kQ8>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kStageSmemBudget) != cudaSuccess)
       return NVATTN_ERR_CUDA;
@@ -495,20 +557,16 @@ nvattn_status launch_staged(const KvStoreParams& p, const StagedPlan& plan, int 
   }
   const int grid = std::min(sm_count, plan.n_chunks);
   const size_t smem = kStageHeader + (size_t)plan.n_stages * plan.stage_bytes;
-  kv_store_staged_kernel<kQOut>
+  kv_store_staged_kernel<kQOut, kQ8>
       <<<grid, (plan.consumer_warps + 1) * 32, smem, stream>>>(p, plan);
   return cudaGetLastError() == cudaSuccess ? NVATTN_OK : NVATTN_ERR_CUDA;
 }
 
-}  // namespace
-
-nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const float* q,
-                              const float* k, const float* v, const uint16_t* qw,
-                              const uint16_t* kw, const int32_t* positions,
-                              const int32_t* slots, void* q_out, nvattn_dtype q_out_dtype,
-                              uint16_t* k_cache, uint16_t* v_cache, uint16_t* k_rows,
-                              uint16_t* v_rows, cudaStream_t stream) {
-  if (n_tokens == 0) return NVATTN_OK;
+// Everything but the destination of the K and V rows, for both cache types.
+KvStoreParams store_params(nvattn_handle* h, int layer, int n_tokens, const float* q,
+                           const float* k, const float* v, const uint16_t* qw,
+                           const uint16_t* kw, const int32_t* positions, const int32_t* slots,
+                           void* q_out, uint16_t* k_rows, uint16_t* v_rows) {
   KvStoreParams p = {};
   p.n_tokens = n_tokens;
   p.Hq = h->cfg.n_q_heads;
@@ -522,11 +580,16 @@ nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const f
   p.slots = slots;
   p.rope = h->rope_table_dev;
   p.q_out = q_out;
-  p.k_cache = k_cache;
-  p.v_cache = v_cache;
   p.k_rows = k_rows;
   p.v_rows = v_rows;
   p.status = h->status_dev;
+  return p;
+}
+
+template <bool kQ8>
+nvattn_status launch_store(nvattn_handle* h, KvStoreParams p, nvattn_dtype q_out_dtype,
+                           cudaStream_t stream) {
+  const int n_tokens = p.n_tokens;
   const long long rows = (long long)n_tokens * (p.Hq + 2 * p.Hkv);
   if (rows > 0x7fffffffLL - kMaxRowsPerGroup * kGroupsPerBlock) return NVATTN_ERR_INVALID_ARG;
   p.total_rows = (int)rows;
@@ -541,9 +604,9 @@ nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const f
   if (plan.n_stages >= 3 && plan.n_chunks >= 4 * h->sm_count) {
     p.rows_per_group = 0;
     switch (q_kind) {
-      case kQOutBf16: return launch_staged<kQOutBf16>(p, plan, h->sm_count, stream);
-      case kQOutF16: return launch_staged<kQOutF16>(p, plan, h->sm_count, stream);
-      default: return launch_staged<kQOutF32>(p, plan, h->sm_count, stream);
+      case kQOutBf16: return launch_staged<kQOutBf16, kQ8>(p, plan, h->sm_count, stream);
+      case kQOutF16: return launch_staged<kQOutF16, kQ8>(p, plan, h->sm_count, stream);
+      default: return launch_staged<kQOutF32, kQ8>(p, plan, h->sm_count, stream);
     }
   }
   // One wave: as many groups as the resident blocks hold (the occupancy of
@@ -560,7 +623,8 @@ nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const f
     if (per_sm[one] <= 0) {
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(
               &per_sm[one],
-              one ? kv_store_rows_kernel<kQOutF32, true> : kv_store_rows_kernel<kQOutF32, false>,
+              one ? kv_store_rows_kernel<kQOutF32, true, kQ8>
+                  : kv_store_rows_kernel<kQOutF32, false, kQ8>,
               kThreads, 0) != cudaSuccess)
         return NVATTN_ERR_CUDA;
       per_sm[one] = std::max(1, per_sm[one]);
@@ -576,18 +640,52 @@ nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const f
   auto launch = [&](auto kernel) { kernel<<<blocks, kThreads, 0, stream>>>(p); };
   switch (q_kind) {
     case kQOutBf16:
-      one_row ? launch(kv_store_rows_kernel<kQOutBf16, true>)
-              : launch(kv_store_rows_kernel<kQOutBf16, false>);
+      one_row ? launch(kv_store_rows_kernel<kQOutBf16, true, kQ8>)
+              : launch(kv_store_rows_kernel<kQOutBf16, false, kQ8>);
       break;
     case kQOutF16:
-      one_row ? launch(kv_store_rows_kernel<kQOutF16, true>)
-              : launch(kv_store_rows_kernel<kQOutF16, false>);
+      one_row ? launch(kv_store_rows_kernel<kQOutF16, true, kQ8>)
+              : launch(kv_store_rows_kernel<kQOutF16, false, kQ8>);
       break;
     default:
-      one_row ? launch(kv_store_rows_kernel<kQOutF32, true>)
-              : launch(kv_store_rows_kernel<kQOutF32, false>);
+      one_row ? launch(kv_store_rows_kernel<kQOutF32, true, kQ8>)
+              : launch(kv_store_rows_kernel<kQOutF32, false, kQ8>);
   }
   return cudaGetLastError() == cudaSuccess ? NVATTN_OK : NVATTN_ERR_CUDA;
+}
+
+}  // namespace
+
+nvattn_status launch_kv_store(nvattn_handle* h, int layer, int n_tokens, const float* q,
+                              const float* k, const float* v, const uint16_t* qw,
+                              const uint16_t* kw, const int32_t* positions,
+                              const int32_t* slots, void* q_out, nvattn_dtype q_out_dtype,
+                              uint16_t* k_cache, uint16_t* v_cache, uint16_t* k_rows,
+                              uint16_t* v_rows, cudaStream_t stream) {
+  if (n_tokens == 0) return NVATTN_OK;
+  KvStoreParams p = store_params(h, layer, n_tokens, q, k, v, qw, kw, positions, slots, q_out,
+                                 k_rows, v_rows);
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  return launch_store<false>(h, p, q_out_dtype, stream);
+}
+
+nvattn_status launch_kv_store_q8(nvattn_handle* h, int layer, int n_tokens, const float* q,
+                                 const float* k, const float* v, const uint16_t* qw,
+                                 const uint16_t* kw, const int32_t* positions,
+                                 const int32_t* slots, void* q_out, nvattn_dtype q_out_dtype,
+                                 uint8_t* k_q8, float* k_scale, uint8_t* v_q8, float* v_scale,
+                                 uint16_t* k_rows, uint16_t* v_rows, cudaStream_t stream) {
+  if (n_tokens == 0) return NVATTN_OK;
+  KvStoreParams p = store_params(h, layer, n_tokens, q, k, v, qw, kw, positions, slots, q_out,
+                                 k_rows, v_rows);
+  p.block_size = h->cfg.block_size;
+  p.num_blocks = h->cfg.num_blocks;
+  p.k_q8 = k_q8;
+  p.v_q8 = v_q8;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  return launch_store<true>(h, p, q_out_dtype, stream);
 }
 
 }  // namespace nvattn

@@ -1,0 +1,77 @@
+// tile_split.cuh -- an even split of a ragged batch's key tiles over a grid.
+//
+// A unit is one (sequence, kv head [, row tile]) and has the key tiles of its
+// sequence, at least one (a unit without keys still writes its rows).  The
+// units' tiles, sequence after sequence, form one line that is cut into equal
+// runs of `per` tiles, one run per CTA: every CTA reads the same number of
+// bytes however ragged the contexts are, a unit that lies inside a run needs
+// no merge, and a run touches at most two units that others share.  Each CTA
+// finds its run from the context lengths themselves (no host work, so a
+// captured launch follows new lengths), every warp for itself (no barrier).
+#pragma once
+
+#include "common.cuh"
+
+namespace nvattn {
+namespace tilesplit {
+
+struct Run {
+  long long begin, end;  // global tile indexes of this CTA's run
+  long long per;         // tiles per CTA
+  int seq;               // sequence that holds `begin`
+  long long seq_first;   // global index of that sequence's first tile
+};
+
+// Shape of one sequence: `units` units of `tiles` key tiles each.
+struct SeqTiles {
+  int units, tiles;
+};
+
+// Warp-collective.  shape(s) gives sequence s's SeqTiles.
+template <class Shape>
+__device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, Shape shape) {
+  const int lane = threadIdx.x & 31;
+  long long sum = 0;
+  for (int s = lane; s < n_seqs; s += 32) {
+    const SeqTiles t = shape(s);
+    sum += (long long)t.units * t.tiles;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  Run r;
+  r.per = (sum + n_ctas - 1) / n_ctas;
+  r.begin = (long long)cta * r.per;
+  r.end = min(sum, r.begin + r.per);
+  r.seq = 0;
+  r.seq_first = 0;
+  if (r.begin >= sum) {
+    r.end = r.begin;
+    return r;
+  }
+  long long before = 0;
+  for (int base = 0; base < n_seqs; base += 32) {
+    long long mine = 0;
+    if (base + lane < n_seqs) {
+      const SeqTiles t = shape(base + lane);
+      mine = (long long)t.units * t.tiles;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + incl > r.begin);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      r.seq = base + l;
+      r.seq_first = before + __shfl_sync(0xffffffffu, incl - mine, l);
+      return r;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return r;
+}
+
+}  // namespace tilesplit
+}  // namespace nvattn

@@ -34,7 +34,7 @@ EXPORTED = [
     "nvattn_sample", "nvattn_schedule_prefill_chunks", "nvattn_kv_store_qk_norm_rope_rows",
     "nvattn_paged_prefill_rows", "nvattn_paged_decode_step", "nvattn_paged_decode_step_launches",
     "nvattn_gather_init", "nvattn_gather_connect", "nvattn_paged_decode_step_gather",
-    "nvattn_gather_read",
+    "nvattn_gather_read", "nvattn_kv_store_q8", "nvattn_kv_load_q8", "nvattn_paged_decode_q8",
 ]
 IPC_HANDLE_BYTES = 128
 ERR_SCRATCH_LIMIT = 7
@@ -123,6 +123,12 @@ def lib():
                                            _i32, _vp, _vp, _vp, _vp]
         L.nvattn_paged_decode_noalloc.argtypes = [ctypes.POINTER(Config), _i32, _i32, _vp, _vp,
                                                   _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp]
+        L.nvattn_kv_store_q8.argtypes = [_vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                         _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
+        L.nvattn_kv_load_q8.argtypes = [_vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp,
+                                        _vp]
+        L.nvattn_paged_decode_q8.argtypes = [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
+                                             _i32, _vp, _i32, _vp, _vp]
         # every other entry point returns nvattn_status (ctypes' default c_int)
         _lib = L
     return _lib
@@ -166,6 +172,30 @@ def _stream_ptr(stream):
     if stream is None:
         return None
     return _vp(int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream))
+
+
+def _addr(t):
+    """Raw address of a tensor, or None, as ctypes takes it for a pointer."""
+    return None if t is None else t.data_ptr()
+
+
+def _stream_addr(stream):
+    return None if stream is None else getattr(stream, "cuda_stream", stream)
+
+
+_dtypes = None
+
+
+def _dtype(t):
+    """NVATTN_DTYPE_* of a float tensor (a type without one raises)."""
+    global _dtypes
+    if _dtypes is None:
+        import torch
+        _dtypes = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+    d = _dtypes.get(t.dtype)
+    if d is None:
+        raise TypeError(f"unsupported type {t.dtype}")
+    return d
 
 
 class Handle:
@@ -337,6 +367,49 @@ class Handle:
                                                  _stream_ptr(stream))
         if check:
             _check(st, "nvattn_paged_prefill")
+        return st
+
+
+    # ---- 8-bit paged cache: payload [n_layer][num_blocks][Hkv][block_size][128]
+    # uint8 (or float8_e4m3fn), scale [n_layer][num_blocks][Hkv][block_size] f32 ----
+    def kv_store_q8(self, layer, q, k, v, q_norm_w, k_norm_w, positions, slots, q_out, k_q8,
+                    k_scale, v_q8, v_scale, stream=None, check=True, k_rows=None, v_rows=None):
+        """nvattn_kv_store_q8: kv_store into the 8-bit cache."""
+        st = lib().nvattn_kv_store_q8(
+            self._h, layer, positions.shape[0], _addr(q), _addr(k), _addr(v), _addr(q_norm_w),
+            _addr(k_norm_w), _addr(positions), _addr(slots), _addr(q_out), _dtype(q_out),
+            _addr(k_q8), _addr(k_scale), _addr(v_q8), _addr(v_scale), _addr(k_rows),
+            _addr(v_rows), _stream_addr(stream))
+        if check:
+            _check(st, "nvattn_kv_store_q8")
+        return st
+
+    def kv_load_q8(self, layer, slots, k_q8, k_scale, v_q8, v_scale, k_out, v_out, stream=None,
+                   check=True):
+        """nvattn_kv_load_q8: the slots' rows into k_out / v_out
+        [n_tokens][Hkv][128] (f32, bf16 or f16, the same for both)."""
+        if k_out.dtype != v_out.dtype:
+            raise ValueError("k_out and v_out differ in type")
+        st = lib().nvattn_kv_load_q8(
+            self._h, layer, slots.shape[0], _addr(slots), _addr(k_q8), _addr(k_scale),
+            _addr(v_q8), _addr(v_scale), _dtype(k_out), _addr(k_out), _addr(v_out),
+            _stream_addr(stream))
+        if check:
+            _check(st, "nvattn_kv_load_q8")
+        return st
+
+    def decode_q8(self, layer, q, k_q8, k_scale, v_q8, v_scale, block_tables, context_lens,
+                  max_context_len, out, stream=None, check=True):
+        """nvattn_paged_decode_q8: q and out f32 or bf16, the same for both."""
+        if q.dtype != out.dtype:
+            raise ValueError("q and out differ in type")
+        st = lib().nvattn_paged_decode_q8(
+            self._h, layer, context_lens.shape[0], _addr(q), _dtype(q), _addr(k_q8),
+            _addr(k_scale), _addr(v_q8), _addr(v_scale), _addr(block_tables),
+            block_tables.shape[1], _addr(context_lens), int(max_context_len), _addr(out),
+            _stream_addr(stream))
+        if check:
+            _check(st, "nvattn_paged_decode_q8")
         return st
 
 
