@@ -50,9 +50,12 @@ constexpr int kStep = 32;                // tokens per warp step
 constexpr int kTile = kWarps * kStep;    // tokens per CTA tile
 constexpr int kStages = 2;
 constexpr int kRows = 8;                 // query rows per unit (GQA group, padded)
+// A unit's start and end (its queries, the warps' merge, its rows or partial)
+// cost about as much as this many tiles, and the split counts them as such.
+constexpr int kUnitCost = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;           // log2: rescale only past 2^8
-static_assert(kTile == 128, "a tile must not cross a block (block sizes are multiples of 128)");
+static_assert(128 % kStep == 0, "a step must not cross a block (block sizes are multiples of 128)");
 
 struct Q8Params {
   int Hq, Hkv, G, layer, block_size, max_blocks, n_seqs, max_context;
@@ -79,7 +82,7 @@ struct __align__(1024) Q8Smem {
   float ks[kWarps][kStages][kStep];
   float vs[kWarps][kStages][kStep];
   float4 tok[kWarps][kStep];  // {score factor, log2 s_v, 1 / s_v, 0} of the step's tokens
-  float o[kWarps][kRows][kD];
+  float o[kWarps][kWarps][kD];  // of the rows being merged
   float m[kWarps][kRows], l[kWarps][kRows];
   uint64_t full[kWarps][kStages];
   int abort_flag;
@@ -88,8 +91,7 @@ struct __align__(1024) Q8Smem {
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -109,6 +111,7 @@ __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint
 struct Walk {
   long long at;  // global tile index
   int seq, head, tile, ctx, n_tiles;
+  int block, offset;  // where this warp's step of the tile lies in the sequence
 };
 
 __device__ __forceinline__ int clamped_ctx(const Q8Params& p, int seq) {
@@ -118,8 +121,20 @@ __device__ __forceinline__ int tiles_of(int ctx) { return max(1, (ctx + kTile - 
 
 __device__ __forceinline__ void walk_next(const Q8Params& p, long long end, Walk& w) {
   ++w.at;
+  w.offset += kTile;
+  while (w.offset >= p.block_size) {
+    w.offset -= p.block_size;
+    ++w.block;
+  }
   if (++w.tile < w.n_tiles) return;
+  w.at += kUnitCost;
   w.tile = 0;
+  w.block = 0;
+  w.offset = (threadIdx.x >> 5) * kStep;
+  while (w.offset >= p.block_size) {
+    w.offset -= p.block_size;
+    ++w.block;
+  }
   if (++w.head < p.Hkv) return;
   w.head = 0;
   ++w.seq;
@@ -186,19 +201,71 @@ __device__ __forceinline__ float load_q(const Q8Params& p, int seq, int head, in
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
+// Dims [4 * lane, 4 * lane + 4) of query row `row` of the unit.
 template <bool kBf16>
-__device__ __forceinline__ void write_out(const Q8Params& p, int seq, int head, int row, int d,
-                                          float o, float l) {
-  const float y = l == 0.0f ? 0.0f : o / l;  // no key: zeros
-  const long long i = ((long long)seq * p.Hq + (long long)head * p.G + row) * kD + d;
+__device__ __forceinline__ void write_out(const Q8Params& p, int seq, int head, int row, int lane,
+                                          const float4& o, float l) {
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+  const float4 y = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+  const long long i = ((long long)seq * p.Hq + (long long)head * p.G + row) * kD + 4 * lane;
   if constexpr (kBf16)
-    static_cast<uint16_t*>(p.out)[i] = (uint16_t)f32_to_bf16_bits(y);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + i) =
+        make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
   else
-    static_cast<float*>(p.out)[i] = y;
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + i) = y;
+}
+
+__device__ __forceinline__ void fma4(float4& o, const float4& a, float f) {
+  o.x = fmaf(a.x, f, o.x);
+  o.y = fmaf(a.y, f, o.y);
+  o.z = fmaf(a.z, f, o.z);
+  o.w = fmaf(a.w, f, o.w);
+}
+
+// Merges the partials of a unit that CTAs c0..c1 share, in CTA order.  A warp
+// per row, 32 partials at a time: a lane per partial for the factors, then
+// four dimensions per lane, the partials' loads independent of one another.
+template <bool kBf16>
+__device__ __forceinline__ void merge_parts(const Q8Params& p, int seq, int head, int c0, int c1) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < p.G; r += kWarps) {
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float M = -INFINITY, L = 0.0f;
+    for (int base = c0; base <= c1; base += 32) {
+      const int n = min(c1 + 1 - base, 32);
+      // (the first CTA left its part in its second place: tile_split.cuh)
+      const float* q = p.part + ((long long)base * 2 + (base == c0)) * kQ8PartFloats;
+      const long long step = 2 * kQ8PartFloats - (base == c0 ? kQ8PartFloats : 0);
+      auto at = [&](int i) {
+        return i == 0 ? q : q + step + (long long)(i - 1) * 2 * kQ8PartFloats;
+      };
+      float m = -INFINITY, l = 0.0f;
+      if (lane < n) {
+        m = __ldcg(at(lane) + kRows * kD + r);
+        l = __ldcg(at(lane) + kRows * kD + kRows + r);
+      }
+      float top = fmaxf(m, M);
+#pragma unroll
+      for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+      const float old = M == -INFINITY ? 1.0f : fast_exp2(M - top);
+      const float f = m == -INFINITY ? 1.0f : fast_exp2(m - top);
+      float s = l * f;
+#pragma unroll
+      for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      L = fmaf(L, old, s);
+      M = top;
+      O = make_float4(O.x * old, O.y * old, O.z * old, O.w * old);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i)
+        fma4(O, __ldcg(reinterpret_cast<const float4*>(at(i) + r * kD) + lane),
+             __shfl_sync(0xffffffffu, f, i));
+    }
+    write_out<kBf16>(p, seq, head, r, lane, O, L);
+  }
 }
 
 template <bool kBf16>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
     decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, Q8Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -219,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   volatile int* abort_flag = &sm.abort_flag;
   const tilesplit::Run run =
       tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, [&](int s) {
-        return tilesplit::SeqTiles{p.Hkv, tiles_of(clamped_ctx(p, s))};
+        return tilesplit::SeqTiles{p.Hkv, tiles_of(clamped_ctx(p, s)) + kUnitCost};
       });
   __syncthreads();
   if (run.begin >= run.end || sm.last) return;
@@ -229,8 +296,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   w.seq = run.seq;
   w.ctx = clamped_ctx(p, w.seq);
   w.n_tiles = tiles_of(w.ctx);
-  w.head = (int)((run.begin - run.seq_first) / w.n_tiles);
-  w.tile = (int)((run.begin - run.seq_first) % w.n_tiles);
+  w.head = (int)((run.begin - run.seq_first) / (w.n_tiles + kUnitCost));
+  w.tile = (int)((run.begin - run.seq_first) % (w.n_tiles + kUnitCost)) - kUnitCost;
+  if (w.tile < 0) {  // the run begins before a unit's first tile
+    w.at -= w.tile;
+    w.tile = 0;
+    if (w.at >= run.end) return;
+  }
+  w.block = (w.tile * kTile + warp * kStep) / p.block_size;
+  w.offset = (w.tile * kTile + warp * kStep) % p.block_size;
 
   // ---- loads: one step = this warp's 32 tokens of a tile ----
   Walk ahead = w;
@@ -239,14 +313,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto block_of = [&](const Walk& x) -> int {
     const int t0 = x.tile * kTile + warp * kStep;
     if (x.at >= run.end || t0 >= x.ctx) return 0;
-    return p.block_tables[(long long)x.seq * p.max_blocks + t0 / p.block_size];
+    return p.block_tables[(long long)x.seq * p.max_blocks + x.block];
   };
   int next_bid = block_of(ahead);
   auto issue = [&]() {  // the step at `ahead`, if it has tokens; moves `ahead` on
     const int t0 = ahead.tile * kTile + warp * kStep;
     const bool some = t0 < ahead.ctx;
     long long bid = next_bid;
-    const int head = ahead.head;
+    const int head = ahead.head, offset = ahead.offset;
     const int seq = ahead.seq, raw = ahead.tile == 0 && ahead.head == 0;
     walk_next(p, run.end, ahead);
     next_bid = block_of(ahead);  // used a step later: its latency is off the path
@@ -264,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int st = issued % kStages;
       uint64_t* bar = &sm.full[warp][st];
       const int page = (int)((long long)p.layer * p.num_blocks + bid);
-      const int row = head * p.block_size + t0 % p.block_size;
+      const int row = head * p.block_size + offset;
       const long long srow = (long long)page * p.Hkv * p.block_size + row;
       mbar_arrive_expect_tx(bar, 2 * kStep * (kD + 4));
       tma_load_3d_hint(sm.ring[warp].k[st], &tm_k, bar, 0, row, page, policy);
@@ -324,24 +398,34 @@ __global__ void __launch_bounds__(kThreads, 2)
           sm.tok[warp][lane] = f;
           __syncwarp();
         }
-        // ---- scores: 4 tiles of 8 tokens ----
+        // ---- scores: 4 tiles of 8 tokens, their product chains interleaved ----
+        float s[4][4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t u[4][4];
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt) {
+            const uint4 v = *reinterpret_cast<const uint4*>(kt + (8 * nt + pr) * kD +
+                                                            (((c + 4 * hf) ^ pr) << 4));
+            u[nt][0] = v.x; u[nt][1] = v.y; u[nt][2] = v.z; u[nt][3] = v.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+              mma_f16(s[nt], qa[4 * hf + i], e4m3x2_to_f16x2(u[nt][i] & 0xffffu),
+                      e4m3x2_to_f16x2(u[nt][i] >> 16));
+        }
         float x[4][2], inv[4][2];
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
-          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const uint8_t* row = kt + (8 * nt + pr) * kD;
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const uint4 v = *reinterpret_cast<const uint4*>(row + (((c + 4 * hf) ^ pr) << 4));
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma_f16(s, qa[4 * hf + i], e4m3x2_to_f16x2(u[i] & 0xffffu),
-                      e4m3x2_to_f16x2(u[i] >> 16));
-          }
           const float4 f0 = sm.tok[warp][8 * nt + c], f1 = sm.tok[warp][8 * nt + c + 4];
-          x[nt][0] = fmaf((s[0] + s[2]) * up, f0.x, f0.y);
-          x[nt][1] = fmaf((s[1] + s[3]) * up, f1.x, f1.y);
+          x[nt][0] = fmaf((s[nt][0] + s[nt][2]) * up, f0.x, f0.y);
+          x[nt][1] = fmaf((s[nt][1] + s[nt][3]) * up, f1.x, f1.y);
           inv[nt][0] = f0.z;
           inv[nt][1] = f1.z;
         }
@@ -363,9 +447,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         uint32_t wa[2][4];
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
-          // x = -inf gives 0 unless no key has been seen (m = -inf too)
-          const float w0 = x[nt][0] == -INFINITY ? 0.0f : fast_exp2(x[nt][0] - m);
-          const float w1 = x[nt][1] == -INFINITY ? 0.0f : fast_exp2(x[nt][1] - m);
+          // (a step has a key: m is -inf only where every key's score is NaN)
+          const float w0 = fast_exp2(x[nt][0] - m), w1 = fast_exp2(x[nt][1] - m);
           l = fmaf(w0, inv[nt][0], l);
           l = fmaf(w1, inv[nt][1], l);
           split_f16(w0, w1, wa[nt >> 1][2 * (nt & 1)], wa[nt >> 1][2 * (nt & 1) + 1]);
@@ -399,49 +482,49 @@ __global__ void __launch_bounds__(kThreads, 2)
       ++done;
     } while (w.at < run.end && w.tile != 0);
 
-    // ---- merge the warps (thread = dimension) ----
+    // ---- merge the warps: a warp per row, four dimensions per lane ----
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (c == 0) {
       sm.m[warp][g] = m;
       sm.l[warp][g] = l;
     }
-    if (g < p.G) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float4 a, b;
-        a = make_float4(o[4 * j][0] + o[4 * j][2], o[4 * j + 1][0] + o[4 * j + 1][2],
-                        o[4 * j + 2][0] + o[4 * j + 2][2], o[4 * j + 3][0] + o[4 * j + 3][2]);
-        b = make_float4(o[4 * j][1] + o[4 * j][3], o[4 * j + 1][1] + o[4 * j + 1][3],
-                        o[4 * j + 2][1] + o[4 * j + 2][3], o[4 * j + 3][1] + o[4 * j + 3][3]);
-        *reinterpret_cast<float4*>(&sm.o[warp][g][16 * c + 4 * j]) = a;
-        *reinterpret_cast<float4*>(&sm.o[warp][g][64 + 16 * c + 4 * j]) = b;
-      }
-    }
-    __syncthreads();
     const bool whole = first == 0 && done == n_tiles;
-    const int d = threadIdx.x;
     float* part = p.part + ((long long)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * kQ8PartFloats;
-    for (int r = 0; r < p.G; ++r) {
-      float M = -INFINITY;
+    for (int r0 = 0; r0 < p.G; r0 += kWarps) {
+      if (g >= r0 && g < min(p.G, r0 + kWarps)) {
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.m[i][r]);
-      float O = 0.0f, L = 0.0f;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const float f = sm.m[i][r] == -INFINITY ? 1.0f : fast_exp2(sm.m[i][r] - M);
-        O = fmaf(sm.o[i][r][d], f, O);
-        L = fmaf(sm.l[i][r], f, L);
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float4*>(&sm.o[warp][g - r0][64 * e + 16 * c + 4 * j]) =
+                make_float4(o[4 * j][e] + o[4 * j][e + 2], o[4 * j + 1][e] + o[4 * j + 1][e + 2],
+                            o[4 * j + 2][e] + o[4 * j + 2][e + 2],
+                            o[4 * j + 3][e] + o[4 * j + 3][e + 2]);
       }
-      if (whole) {
-        write_out<kBf16>(p, seq, head, r, d, O, L);
-      } else {
-        part[r * kD + d] = O;
-        if (d == 0) {
-          part[kRows * kD + r] = M;
-          part[kRows * kD + kRows + r] = L;
+      __syncthreads();
+      if (const int r = r0 + warp; r < p.G) {
+        float M = -INFINITY, L = 0.0f;
+        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.m[i][r]);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          const float f = sm.m[i][r] == -INFINITY ? 1.0f : fast_exp2(sm.m[i][r] - M);
+          fma4(O, *reinterpret_cast<const float4*>(&sm.o[i][warp][4 * lane]), f);
+          L = fmaf(sm.l[i][r], f, L);
+        }
+        if (whole) {
+          write_out<kBf16>(p, seq, head, r, lane, O, L);
+        } else {
+          *reinterpret_cast<float4*>(part + r * kD + 4 * lane) = O;
+          if (lane == 0) {
+            part[kRows * kD + r] = M;
+            part[kRows * kD + kRows + r] = L;
+          }
         }
       }
+      __syncthreads();  // the merge buffer is free
     }
     if (!whole) {
       const int c0 = (int)(unit0 / run.per), c1 = (int)((unit0 + n_tiles - 1) / run.per);
@@ -455,24 +538,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncthreads();
       if (sm.last) {
         __threadfence();
-        for (int r = 0; r < p.G; ++r) {
-          float M = -INFINITY;
-          for (int i = c0; i <= c1; ++i)
-            M = fmaxf(M, __ldcg(p.part + ((long long)i * 2 + (i == c0)) * kQ8PartFloats +
-                                kRows * kD + r));
-          float O = 0.0f, L = 0.0f;
-          for (int i = c0; i <= c1; ++i) {
-            const float* q = p.part + ((long long)i * 2 + (i == c0)) * kQ8PartFloats;
-            const float mi = __ldcg(q + kRows * kD + r);
-            const float f = mi == -INFINITY ? 1.0f : fast_exp2(mi - M);
-            O = fmaf(__ldcg(q + r * kD + d), f, O);
-            L = fmaf(__ldcg(q + kRows * kD + kRows + r), f, L);
-          }
-          write_out<kBf16>(p, seq, head, r, d, O, L);
-        }
+        merge_parts<kBf16>(p, seq, head, c0, c1);
       }
+      __syncthreads();  // sm.last is free
     }
-    __syncthreads();  // the merge buffers are free
   }
   // After a wait that ran out, copies may still be in flight: wait (bounded)
   // for the ring's last ones before the CTA's shared memory goes away.
@@ -516,7 +585,7 @@ nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, co
   p.tickets = h->part_tickets;
   p.status = h->status_dev;
   const size_t smem = sizeof(Q8Smem) + 1024;
-  static_assert(sizeof(Q8Smem) + 1024 <= 113 * 1024, "two CTAs per SM");
+  static_assert(kQ8CtasPerSm * (sizeof(Q8Smem) + 2048) <= 228 * 1024, "CTAs per SM");
   // (atomic: handles on different threads may launch at the same time)
   static std::atomic<unsigned long long> attr_set_mask{0};
   int dev = 0;

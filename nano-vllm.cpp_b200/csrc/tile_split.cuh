@@ -1,11 +1,16 @@
 // tile_split.cuh -- an even split of a ragged batch's key tiles over a grid.
 //
 // A unit is one (sequence, kv head [, row tile]) and has the key tiles of its
-// sequence, at least one (a unit without keys still writes its rows).  The
-// units' tiles, sequence after sequence, form one line that is cut into equal
-// runs of `per` tiles, one run per CTA: every CTA reads the same number of
-// bytes however ragged the contexts are, a unit that lies inside a run needs
-// no merge, and a run touches at most two units that others share.  Each CTA
+// sequence, at least one (a unit without keys still writes its rows), after a
+// fixed number of empty places for what a unit costs besides its tiles.  The
+// units' places, sequence after sequence, form one line that is cut into equal
+// runs of `per` places, one run per CTA: every CTA has the same work however
+// ragged the contexts are, a unit whose tiles lie inside a run needs no merge,
+// and a run touches at most two units that others share.  (A line of tiles
+// alone gave runs of many short units to some CTAs: 47 us instead of 9 for 23
+// sequences of 1 to 9,001 tokens.)  A unit's part from the first CTA that has
+// tiles of it is that CTA's last, every later one's its first; hence two
+// places for partials per CTA.  Each CTA
 // finds its run from the context lengths themselves (no host work, so a
 // captured launch follows new lengths), every warp for itself (no barrier).
 #pragma once
@@ -16,13 +21,13 @@ namespace nvattn {
 namespace tilesplit {
 
 struct Run {
-  long long begin, end;  // global tile indexes of this CTA's run
-  long long per;         // tiles per CTA
+  long long begin, end;  // places of this CTA's run
+  long long per;         // places per CTA
   int seq;               // sequence that holds `begin`
-  long long seq_first;   // global index of that sequence's first tile
+  long long seq_first;   // that sequence's first place
 };
 
-// Shape of one sequence: `units` units of `tiles` key tiles each.
+// Shape of one sequence: `units` units of `tiles` places each.
 struct SeqTiles {
   int units, tiles;
 };
