@@ -232,6 +232,29 @@ NVATTN_API nvattn_status nvattn_sample(
     const int64_t* history_offsets_dev, const float* uniforms_dev, int32_t* tokens_dev,
     nvattn_stream_t stream);
 
+/* ---- log-probabilities ----------------------------------------------------- */
+
+/* Per row of logits (n_vocab values of dtype, f32 or bf16, at
+ * logits_dev + r * row_stride elements; any row_stride >= n_vocab):
+ *   logprobs_dev[r]  log softmax(x)[tokens_dev[r]]
+ *   ranks_dev[r]     how many ids precede tokens_dev[r] in the order (logit
+ *                    descending, id ascending); 0: the greedy choice
+ *   entropy_dev[r]   -sum p log p, in nats (a logit of -inf adds nothing)
+ *   top_ids_dev, top_logprobs_dev [n_rows][top_k]: the first top_k ids of that
+ *                    order and their log-probabilities, top_k <= 64
+ * logprobs_dev, ranks_dev and entropy_dev may be NULL (not computed);
+ * tokens_dev may be NULL when logprobs_dev and ranks_dev are; the top_* may be
+ * NULL when top_k is 0.  A token outside [0, n_vocab) is reported as
+ * NVATTN_ERR_OUT_OF_RANGE (detail = r), its row's logprob is NaN and its rank
+ * -1.  In the order a NaN counts as -inf and -0 equals +0; a row with a NaN, a
+ * +inf or nothing but -inf has NaN log-probabilities and entropy, as the
+ * formulas give.  n_vocab <= 2,097,152.  One launch, no workspace. */
+NVATTN_API nvattn_status nvattn_token_logprobs(
+    nvattn_handle* h, int n_rows, int n_vocab, const void* logits_dev, nvattn_dtype dtype,
+    int64_t row_stride, const int32_t* tokens_dev, float* logprobs_dev, float* entropy_dev,
+    int32_t* ranks_dev, int top_k, int32_t* top_ids_dev, float* top_logprobs_dev,
+    nvattn_stream_t stream);
+
 /* ---- device kernels ----------------------------------------------------- */
 
 /* Fused per-head q/k RMSNorm (weight = q_norm / k_norm), NEOX RoPE at

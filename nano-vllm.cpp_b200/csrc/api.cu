@@ -854,4 +854,29 @@ nvattn_status nvattn_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, co
                                         reinterpret_cast<cudaStream_t>(stream));
 }
 
+nvattn_status nvattn_token_logprobs(nvattn_handle* h, int n_rows, int n_vocab,
+                                    const void* logits_dev, nvattn_dtype dtype,
+                                    int64_t row_stride, const int32_t* tokens_dev,
+                                    float* logprobs_dev, float* entropy_dev, int32_t* ranks_dev,
+                                    int top_k, int32_t* top_ids_dev, float* top_logprobs_dev,
+                                    nvattn_stream_t stream) {
+  if (h == nullptr || n_rows < 0 || n_vocab <= 0 || row_stride < n_vocab || top_k < 0 ||
+      top_k > n_vocab || (dtype != NVATTN_DTYPE_F32 && dtype != NVATTN_DTYPE_BF16))
+    return NVATTN_ERR_INVALID_ARG;
+  if (n_vocab > nvattn::kLogprobsMaxVocab || top_k > nvattn::kMaxTop)
+    return NVATTN_ERR_UNSUPPORTED;
+  if (n_rows == 0) return NVATTN_OK;
+  const uintptr_t el = dtype == NVATTN_DTYPE_BF16 ? 2 : 4;
+  if (logits_dev == nullptr || (reinterpret_cast<uintptr_t>(logits_dev) & (el - 1)) != 0 ||
+      (tokens_dev == nullptr && (logprobs_dev != nullptr || ranks_dev != nullptr)) ||
+      (top_k > 0 && (top_ids_dev == nullptr || top_logprobs_dev == nullptr)))
+    return NVATTN_ERR_INVALID_ARG;
+  DeviceGuard guard(h->cfg.device);
+  if (!guard.ok()) return NVATTN_ERR_CUDA;
+  return nvattn::launch_token_logprobs(h, n_rows, n_vocab, logits_dev, dtype, row_stride,
+                                       tokens_dev, logprobs_dev, entropy_dev, ranks_dev, top_k,
+                                       top_ids_dev, top_logprobs_dev,
+                                       reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -198,6 +198,15 @@ nvattn_status launch_plan_decode(nvattn_handle* h, int n_seqs, const int64_t* se
                                  int32_t* context_lens, int32_t* positions,
                                  int32_t* slot_mapping, cudaStream_t stream);
 
+// Log-probabilities of given tokens (logprobs.cu).
+constexpr int kLogprobsMaxVocab = 2097152;  // as the sampler's
+constexpr int kMaxTop = 64;
+nvattn_status launch_token_logprobs(nvattn_handle* h, int n_rows, int n_vocab, const void* logits,
+                                    nvattn_dtype dtype, long long row_stride,
+                                    const int32_t* tokens, float* logprobs, float* entropy,
+                                    int32_t* ranks, int top_k, int32_t* top_ids,
+                                    float* top_logprobs, cudaStream_t stream);
+
 // Token sampler (sample.cu).
 int sample_max_vocab();
 int sample_vocab_granule();      // samp_cap is a multiple of this

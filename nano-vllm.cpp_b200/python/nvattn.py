@@ -35,6 +35,7 @@ EXPORTED = [
     "nvattn_paged_prefill_rows", "nvattn_paged_decode_step", "nvattn_paged_decode_step_launches",
     "nvattn_gather_init", "nvattn_gather_connect", "nvattn_paged_decode_step_gather",
     "nvattn_gather_read", "nvattn_kv_store_q8", "nvattn_kv_load_q8", "nvattn_paged_decode_q8",
+    "nvattn_token_logprobs",
 ]
 IPC_HANDLE_BYTES = 128
 ERR_SCRATCH_LIMIT = 7
@@ -129,6 +130,8 @@ def lib():
                                         _vp]
         L.nvattn_paged_decode_q8.argtypes = [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
                                              _i32, _vp, _i32, _vp, _vp]
+        L.nvattn_token_logprobs.argtypes = [_vp, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _vp, _vp,
+                                            _i32, _vp, _vp, _vp]
         # every other entry point returns nvattn_status (ctypes' default c_int)
         _lib = L
     return _lib
@@ -369,6 +372,22 @@ class Handle:
             _check(st, "nvattn_paged_prefill")
         return st
 
+
+    def token_logprobs(self, logits, tokens=None, logprobs=None, entropy=None, ranks=None,
+                       top_ids=None, top_logprobs=None, stream=None, check=True):
+        """nvattn_token_logprobs: logits [n_rows][n_vocab] f32 or bf16 with
+        unit stride along the vocabulary; top_k is top_ids.shape[1]."""
+        n, V = logits.shape
+        if V > 1 and logits.stride(1) != 1:
+            raise ValueError("logits are not contiguous along the vocabulary")
+        st = lib().nvattn_token_logprobs(
+            self._h, n, V, _addr(logits), _dtype(logits), max(logits.stride(0), V),
+            _addr(tokens), _addr(logprobs), _addr(entropy), _addr(ranks),
+            0 if top_ids is None else top_ids.shape[1], _addr(top_ids), _addr(top_logprobs),
+            _stream_addr(stream))
+        if check:
+            _check(st, "nvattn_token_logprobs")
+        return st
 
     # ---- 8-bit paged cache: payload [n_layer][num_blocks][Hkv][block_size][128]
     # uint8 (or float8_e4m3fn), scale [n_layer][num_blocks][Hkv][block_size] f32 ----

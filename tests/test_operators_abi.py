@@ -11,3 +11,8 @@ def test_q8_entry_points_reject_a_null_handle():
         nvattn.ERR_INVALID_ARG
     assert L.nvattn_paged_decode_q8(None, 0, 1, None, 0, *([None] * 5), 1, None, 1, None,
                                     None) == nvattn.ERR_INVALID_ARG
+
+
+def test_logprobs_rejects_a_null_handle():
+    assert nvattn.lib().nvattn_token_logprobs(None, 1, 10, None, 0, 10, None, None, None, None, 0,
+                                              None, None, None) == nvattn.ERR_INVALID_ARG
