@@ -448,6 +448,38 @@ NVATTN_API nvattn_status nvattn_paged_prefill_rows(
     const uint16_t* k_rows_f16_dev, const uint16_t* v_rows_f16_dev, float* out_dev,
     nvattn_stream_t stream);
 
+/* ---- attention for trees of drafted tokens --------------------------------- */
+
+/* One verification step of speculative decoding over the BF16 cache; the
+ * reference has no counterpart.  Sequence s brings N_s = cu_nodes[s+1] -
+ * cu_nodes[s] drafted tokens, its nodes, whose K/V rows are stored at the last
+ * N_s positions of its context (nvattn_kv_store_qk_norm_rope first; a node's
+ * RoPE position is its depth in the tree, not its place).  Node i attends every
+ * key before the nodes, [0, context_lens[s] - N_s), and node j of its sequence
+ * where bit j % 64 of tree_mask[cu_nodes[s] + i][j / 64] is set -- usually its
+ * ancestors and itself; bits at or past N_s are ignored.
+ *   q_dev, out_dev [n_nodes][n_q_heads][head_dim] in dtype, f32 or bf16: f32
+ *       keeps f32 accuracy throughout; bf16 rounds only the output (softmax
+ *       weights carry 16 bits)
+ *   cu_nodes_dev [n_seqs+1] int32, tree_mask_dev [n_nodes][mask_words] uint64,
+ *       1 <= mask_words <= 4, max_nodes (host bound of N_s) <= 64 * mask_words
+ *   the rest as nvattn_paged_decode
+ * A node that attends nothing gets zeros.  Slots behind a context may hold
+ * anything, and so may the K/V rows of a node that no mask names: a node's K/V
+ * reaches only the rows that attend it (a NaN or an infinity in its V row
+ * makes all of their output NaN).  A sequence without nodes is skipped; one
+ * whose cu_nodes or context_lens are unusable (N_s negative or above max_nodes,
+ * rows outside n_nodes, context_lens[s] outside [N_s, max_context_len]) is
+ * reported as NVATTN_ERR_OUT_OF_RANGE and its rows are not written.
+ * The launch uses the handle's workspace: calls on one handle are issued on
+ * one stream, as for nvattn_paged_decode. */
+NVATTN_API nvattn_status nvattn_paged_tree_decode(
+    nvattn_handle* h, int layer, int n_seqs, int n_nodes, const void* q_dev, nvattn_dtype dtype,
+    const int32_t* cu_nodes_dev, const uint64_t* tree_mask_dev, int mask_words, int max_nodes,
+    const uint16_t* k_cache_dev, const uint16_t* v_cache_dev, const int32_t* block_tables_dev,
+    int max_blocks, const int32_t* context_lens_dev, int max_context_len, void* out_dev,
+    nvattn_stream_t stream);
+
 /* ---- 8-bit paged KV cache ------------------------------------------------ */
 
 /* An alternative to the BF16 cache at about half its size (264 instead of 512

@@ -879,4 +879,36 @@ nvattn_status nvattn_token_logprobs(nvattn_handle* h, int n_rows, int n_vocab,
                                        reinterpret_cast<cudaStream_t>(stream));
 }
 
+nvattn_status nvattn_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, int n_nodes,
+                                       const void* q_dev, nvattn_dtype dtype,
+                                       const int32_t* cu_nodes_dev, const uint64_t* tree_mask_dev,
+                                       int mask_words, int max_nodes, const uint16_t* k_cache_dev,
+                                       const uint16_t* v_cache_dev,
+                                       const int32_t* block_tables_dev, int max_blocks,
+                                       const int32_t* context_lens_dev, int max_context_len,
+                                       void* out_dev, nvattn_stream_t stream) {
+  if (h == nullptr || layer < 0 || layer >= h->cfg.n_layer || n_seqs < 0 ||
+      n_seqs > h->cfg.max_seqs || n_nodes < 0 || max_blocks <= 0 || max_context_len < 0 ||
+      max_context_len > h->cfg.max_context ||
+      (long long)max_context_len > (long long)max_blocks * h->cfg.block_size || mask_words < 1 ||
+      max_nodes < 0 || max_nodes > 64 * mask_words ||
+      (dtype != NVATTN_DTYPE_F32 && dtype != NVATTN_DTYPE_BF16))
+    return NVATTN_ERR_INVALID_ARG;
+  if (mask_words > nvattn::kMaxMaskWords) return NVATTN_ERR_UNSUPPORTED;
+  if (n_seqs == 0 || n_nodes == 0) return NVATTN_OK;
+  const void* ptrs[] = {q_dev, k_cache_dev, v_cache_dev, out_dev};
+  for (const void* p : ptrs)
+    if (p == nullptr || !aligned16(p)) return NVATTN_ERR_INVALID_ARG;
+  if (cu_nodes_dev == nullptr || tree_mask_dev == nullptr ||
+      (reinterpret_cast<uintptr_t>(tree_mask_dev) & 7u) != 0 || block_tables_dev == nullptr ||
+      context_lens_dev == nullptr)
+    return NVATTN_ERR_INVALID_ARG;
+  DeviceGuard guard(h->cfg.device);
+  if (!guard.ok()) return NVATTN_ERR_CUDA;
+  return nvattn::launch_paged_tree_decode(
+      h, layer, n_seqs, n_nodes, q_dev, dtype, cu_nodes_dev, tree_mask_dev, mask_words, max_nodes,
+      k_cache_dev, v_cache_dev, block_tables_dev, max_blocks, context_lens_dev, max_context_len,
+      out_dev, reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -135,10 +135,24 @@ constexpr int kQ8Warps = 4;
 constexpr int kQ8CtasPerSm = 2;
 // one partial: 8 rows of 128, then 8 references and 8 sums
 constexpr int kQ8PartFloats = 8 * 128 + 16;
-// The workspace of the evenly split kernels (ws_part, part_tickets).
+// Attention for trees of drafted tokens (tree_decode.cu), one CTA per SM; a
+// partial: 128 dims x 128 rows, then 128 references and 128 sums.
+constexpr int kMaxMaskWords = 4;  // 256 nodes per sequence
+constexpr int kTreePartFloats = 128 * 128 + 256;
+nvattn_status launch_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, int n_nodes,
+                                       const void* q, nvattn_dtype dtype, const int32_t* cu_nodes,
+                                       const uint64_t* mask, int mask_words, int max_nodes,
+                                       const uint16_t* k_cache, const uint16_t* v_cache,
+                                       const int32_t* block_tables, int max_blocks,
+                                       const int32_t* context_lens, int max_context_len,
+                                       void* out, cudaStream_t stream);
+// The workspace of the evenly split kernels (ws_part, part_tickets): two
+// partials and one ticket per CTA.
 inline size_t part_ticket_count(int sm_count) { return (size_t)kQ8CtasPerSm * sm_count; }
 inline size_t part_floats(int sm_count) {
-  return 2 * part_ticket_count(sm_count) * kQ8PartFloats;
+  const size_t q8 = 2 * part_ticket_count(sm_count) * kQ8PartFloats;
+  const size_t tree = 2 * (size_t)sm_count * kTreePartFloats;
+  return q8 > tree ? q8 : tree;
 }
 nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, const void* q,
                                      nvattn_dtype dtype, const uint8_t* k_q8,

@@ -35,7 +35,7 @@ EXPORTED = [
     "nvattn_paged_prefill_rows", "nvattn_paged_decode_step", "nvattn_paged_decode_step_launches",
     "nvattn_gather_init", "nvattn_gather_connect", "nvattn_paged_decode_step_gather",
     "nvattn_gather_read", "nvattn_kv_store_q8", "nvattn_kv_load_q8", "nvattn_paged_decode_q8",
-    "nvattn_token_logprobs",
+    "nvattn_token_logprobs", "nvattn_paged_tree_decode",
 ]
 IPC_HANDLE_BYTES = 128
 ERR_SCRATCH_LIMIT = 7
@@ -132,6 +132,8 @@ def lib():
                                              _i32, _vp, _i32, _vp, _vp]
         L.nvattn_token_logprobs.argtypes = [_vp, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _vp, _vp,
                                             _i32, _vp, _vp, _vp]
+        L.nvattn_paged_tree_decode.argtypes = [_vp, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32,
+                                               _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp]
         # every other entry point returns nvattn_status (ctypes' default c_int)
         _lib = L
     return _lib
@@ -372,6 +374,23 @@ class Handle:
             _check(st, "nvattn_paged_prefill")
         return st
 
+
+    def tree_decode(self, layer, q, cu_nodes, tree_mask, max_nodes, k_cache, v_cache,
+                    block_tables, context_lens, max_context_len, out, stream=None, check=True):
+        """nvattn_paged_tree_decode: q and out [n_nodes][Hq][128], f32 or bf16,
+        the same for both; tree_mask [n_nodes][mask_words] of 64-bit words."""
+        if q.dtype != out.dtype:
+            raise ValueError("q and out differ in type")
+        if tree_mask.element_size() != 8 or tree_mask.shape[0] < q.shape[0]:
+            raise ValueError("tree_mask holds 64-bit words, a row per node")
+        st = lib().nvattn_paged_tree_decode(
+            self._h, layer, context_lens.shape[0], q.shape[0], _addr(q), _dtype(q),
+            _addr(cu_nodes), _addr(tree_mask), tree_mask.shape[1], int(max_nodes),
+            _addr(k_cache), _addr(v_cache), _addr(block_tables), block_tables.shape[1],
+            _addr(context_lens), int(max_context_len), _addr(out), _stream_addr(stream))
+        if check:
+            _check(st, "nvattn_paged_tree_decode")
+        return st
 
     def token_logprobs(self, logits, tokens=None, logprobs=None, entropy=None, ranks=None,
                        top_ids=None, top_logprobs=None, stream=None, check=True):

@@ -85,13 +85,13 @@ def slots_of(bt_row, n, bs):
     return bt_row[t // bs].astype(np.int64) * bs + t % bs
 
 
-def attend(q, k, v, keep=None, scale=1 / np.sqrt(D)):
+def attend(q, k, v, keep=None, scale=1 / np.sqrt(D), weight_bits=20):
     """Rows q [R][128] over keys [n][128] in 64 bits; keep [R][n] masks.  Also
     the bound on what f32 arithmetic may be off: |dS| of each score is within
     2^-16 of sum|q k| (a 128-term dot product, terms exact or of 22 bits), a
     change of dS moves the output by at most (e^(2 dS) - 1) sum p|v|, the
-    exponential and the weights' 22 bits add 2^-20, and chains of n/16 + 64
-    f32 additions 2^-23 each."""
+    exponential and the weights' bits (22 in the 8-bit decode) add 2^-weight_bits,
+    and chains of n/16 + 64 f32 additions 2^-23 each."""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
     x = q @ k.T * scale
     size = np.abs(q) @ np.abs(k).T * scale
@@ -103,7 +103,7 @@ def attend(q, k, v, keep=None, scale=1 / np.sqrt(D)):
     tot = e.sum(-1, keepdims=True)
     p = e / np.where(tot > 0, tot, 1)
     ds = size.max(-1, keepdims=True, initial=0) * 2.0 ** -16
-    rel = np.expm1(2 * ds) + 2.0 ** -20 + (k.shape[0] / 16 + 64) * 2.0 ** -23
+    rel = np.expm1(2 * ds) + 2.0 ** -weight_bits + (k.shape[0] / 16 + 64) * 2.0 ** -23
     return p @ v, rel * (p @ np.abs(v))
 
 

@@ -16,3 +16,9 @@ def test_q8_entry_points_reject_a_null_handle():
 def test_logprobs_rejects_a_null_handle():
     assert nvattn.lib().nvattn_token_logprobs(None, 1, 10, None, 0, 10, None, None, None, None, 0,
                                               None, None, None) == nvattn.ERR_INVALID_ARG
+
+
+def test_tree_decode_rejects_a_null_handle():
+    assert nvattn.lib().nvattn_paged_tree_decode(None, 0, 1, 1, None, 0, None, None, 1, 1, None,
+                                                 None, None, 1, None, 1, None, None) == \
+        nvattn.ERR_INVALID_ARG
