@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
   }
   volatile int* abort_flag = &sm.abort_flag;
   const tilesplit::Run run =
-      tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, [&](int s) {
+      tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, 1, [&](int s) {
         return tilesplit::SeqTiles{p.Hkv, tiles_of(clamped_ctx(p, s)) + kUnitCost};
       });
   __syncthreads();

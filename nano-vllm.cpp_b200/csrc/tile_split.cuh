@@ -32,9 +32,11 @@ struct SeqTiles {
   int units, tiles;
 };
 
-// Warp-collective.  shape(s) gives sequence s's SeqTiles.
+// Warp-collective.  shape(s) gives sequence s's SeqTiles; runs have at least
+// min_run places (short work then leaves CTAs without any).
 template <class Shape>
-__device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, Shape shape) {
+__device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, int min_run,
+                                        Shape shape) {
   const int lane = threadIdx.x & 31;
   long long sum = 0;
   for (int s = lane; s < n_seqs; s += 32) {
@@ -44,7 +46,7 @@ __device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, Shape s
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   Run r;
-  r.per = (sum + n_ctas - 1) / n_ctas;
+  r.per = max((sum + n_ctas - 1) / n_ctas, (long long)min_run);
   r.begin = (long long)cta * r.per;
   r.end = min(sum, r.begin + r.per);
   r.seq = 0;

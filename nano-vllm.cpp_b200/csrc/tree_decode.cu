@@ -9,27 +9,41 @@
 // sequence is node r / G, query head r % G.  So all nodes and all query heads
 // of a kv head read its keys together: 512 bytes per token and kv head for up
 // to 128 rows, bound by memory until a kv head has several row tiles (whose
-// keys then come from L2).  The units' 64-key tiles are split evenly over one
-// CTA per SM (tile_split.cuh); the partials that this makes are merged by the
-// CTA that finishes a unit last, in CTA order.
+// keys then come from L2).  The units' key tiles (kTile keys) are split evenly
+// over one CTA per SM (tile_split.cuh); the partials
+// that this makes are published at the CTA's end, and the CTA that publishes a
+// unit's last one merges them, in CTA order.
 //
-//   warp 0      TMA producer: K and V tiles of 16 KiB (two boxes of 64 dims x
-//               64 tokens, 128-byte swizzle) through a ring of kSlots that
-//               runs on across units.
-//   warp 1      TMEM allocation; one lane issues the MMAs (M = 128 rows):
-//                 S(j) = Q K^T   N = 64 keys, A = Q from TMEM
-//                 O   += P V     N = 128 dims, K = 64 keys, A = P from TMEM
-//               S(j+1) before P V(j), so that the softmax never waits for the
-//               tensor cores; both A operands come from TMEM, which leaves the
-//               shared-memory reads to K and V.
-//   warps 2-5   thread = row = TMEM lane: queries into TMEM, mask, online
-//               softmax in the log2 domain with lazy rescaling of O, P over
-//               the columns of its own S, epilogue.
+//   warp 0      TMA producer: K and V tiles (two boxes of 64 dims, 128-byte
+//               swizzle) through a ring of slots that runs on across units,
+//               and before a unit's first K tile its bf16 queries (box: 64
+//               dims x G heads x 128 / G nodes, the operand's layout) into one
+//               of two buffers.
+//   warp 1      TMEM allocation; issues S(j) = Q K^T (M = 128 rows, N = kTile
+//               keys), up to kBufs tiles ahead, into the next unit too, so that
+//               a unit's first scores are there when its softmax starts.
+//   warp 2      issues O_w += P V (N = 128 dims, K = kTile keys, A = P from
+//               TMEM).  Two issuers, as one spent more time on the waits and
+//               commits between the MMAs than on the MMAs.
+//   warps 4-11  two groups of four, thread = row = TMEM lane: group w takes
+//               the tiles j with j % 2 = w (counted over the run), with its own
+//               S / P buffer, running maximum, sum and O_w, so the groups never
+//               wait for one another inside a unit, and the tensor cores work
+//               on one group's tile while the other group's softmax runs.
+//               Online softmax in the log2 domain with lazy rescaling of O_w;
+//               P over the columns of its own S.  At a unit's end each group
+//               combines O_0 and O_1 for half of the dims.  f32 queries are
+//               split into their terms by these warps (one buffer).
 // Precision: products of bf16 operands, f32 sums.  bf16 queries are one
 // operand and P is a sum of two bf16 terms (16 bits; one term, 8 bits, would
 // add as much error as the rounding of a bf16 output itself).  f32 queries and
 // their P are sums of three bf16 terms, 24 bits: f32 in, f32 out.
-// TMEM columns: Q [0, 64 kQ), O [192, 320), then two S / P buffers of 96.
+// TMEM columns: O_0 [0, 128), O_1 [128, 256), then the S / P buffers, tile j in
+// buffer j % kBufs: P holds, over each 32 keys' own scores, their first terms
+// and their second terms (16 columns each), the third terms behind the tile's
+// scores.  With four buffers (bf16) a group finds its next scores there while
+// its last P V still runs; with two, score, softmax and P V of a group's tiles
+// follow one another.
 #include <atomic>
 
 #include "common.cuh"
@@ -42,16 +56,26 @@ namespace {
 constexpr int kD = 128;
 constexpr int kRows = 128;
 constexpr int kTile = 64;  // keys per tile
-constexpr int kThreads = 6 * 32;
-constexpr int kSlots = 13;
-constexpr int kHalfBytes = kTile * 64 * 2;  // one box: 64 tokens x 64 dims
+constexpr int kGroup = 128;  // softmax threads of one group
+constexpr int kThreads = 3 * kGroup;
+// Registers per thread: 168 at launch (384 threads); the softmax groups take
+// what warps 0-3 give up: 136 + 2 * 184 = 3 * 168.
+constexpr int kControlRegs = 136, kSoftmaxRegs = 184;
+constexpr int kQTermBytes = kRows * kD * 2;     // [d half][row][64], 128-byte swizzle
+constexpr int kOperandBytes = 13 * 16 * 1024;  // query operands and the ring share it
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColO = 192, kColS = 320, kColsS = 96;
+constexpr uint32_t kColS = 256;  // the S / P buffers; O_0 and O_1 lie before them
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.0f;  // log2: rescale O only when a row's maximum grows past 2^8
-// A unit's start and end cost about as much as this many tiles (its queries
-// into TMEM, the first S and the epilogue do not overlap its neighbours').
-constexpr int kUnitCost = 4;
+// log2: a row's reference moves only when a score passes it by 2^32.  P, O and
+// the sums are floating point, so weights above 1 lose nothing, and f32 leaves
+// 2^90 for the values.
+constexpr float kSlack = 32.0f;
+// A unit's end costs about as much as this many keys, and the split counts
+// them.
+constexpr int kUnitCostKeys = 256;
+// Fewest keys per CTA: below that a CTA's own start and the merge of more
+// partials cost more than the tiles.
+constexpr int kMinRunKeys = 512;
 
 struct TreeParams {
   int Hq, Hkv, G, layer, block_size, max_blocks, n_seqs, n_nodes, max_nodes, mask_words;
@@ -69,20 +93,19 @@ struct TreeParams {
   DeviceStatus* status;
 };
 
+constexpr int kMaxSlots = 13;
 struct __align__(1024) TreeSmem {
-  uint16_t kv[kSlots][2][kTile * 64];  // [slot][d half][token][64]
-  uint64_t full[kSlots], empty[kSlots];
-  uint64_t q_ready, s_full[2], p_full[2], o_done[2];
-  uint32_t bad[2][2];  // [tile & 1]: keys of the tile whose V row holds a NaN or an infinity
+  uint8_t operands[kOperandBytes];  // query terms, then the K / V ring
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t q_full[2], q_empty[2], s_full[4], p_full[4], o_done;
+  float m[2][kRows], l[2][kRows];  // the groups' references and sums at a unit's end
+  uint32_t bad[2][4];  // [group]: keys of its tile whose V row holds a NaN or an infinity
   uint32_t tmem_base;
   int abort_flag;
   int skip;
-  int last;
+  int last[2];
 };
 static_assert(sizeof(TreeSmem) + 1024 <= 227 * 1024, "shared memory");
-
-__device__ __forceinline__ int ring_slot(int idx) { return idx % kSlots; }
-__device__ __forceinline__ uint32_t ring_parity(int idx) { return (uint32_t)(idx / kSlots) & 1u; }
 
 // A sequence's nodes and context; n = 0 where it has none or its metadata is
 // unusable (`report`: recorded then).
@@ -105,7 +128,9 @@ __device__ __forceinline__ SeqInfo seq_info(const TreeParams& p, int s, bool rep
 __device__ __forceinline__ int row_tiles(const TreeParams& p, int n) {
   return (n * p.G + kRows - 1) / kRows;
 }
-__device__ __forceinline__ int key_tiles(int ctx) { return (ctx + kTile - 1) / kTile; }
+__device__ __forceinline__ int key_tiles(int ctx) {
+  return (ctx + kTile - 1) / kTile;
+}
 
 // One unit's part of the CTA's run: key tiles [j0, j1).
 struct Segment {
@@ -116,6 +141,7 @@ struct Segment {
 
 // Walks the segments of a run; every role walks the same ones.
 struct Walker {
+  static constexpr int kUnitCost = kUnitCostKeys / kTile;
   long long at, end, per;
   int seq, unit;  // the unit that `at` lies in
   SeqInfo info;
@@ -163,33 +189,110 @@ struct Walker {
 // The next bf16 term of two values; they keep what is left.
 __device__ __forceinline__ void split_term(float& x0, float& x1, uint32_t& packed) {
   packed = cvt_bf16x2(x0, x1);
-  x0 -= bf16lo_to_f32(packed);
-  x1 -= bf16hi_to_f32(packed);
+  unpack2(fsub2(pack2(x0, x1), pack2(bf16lo_to_f32(packed), bf16hi_to_f32(packed))), x0, x1);
+}
+
+// kN consecutive dims of an output row at element `at`, times f.
+template <bool kF32, int kN>
+__device__ __forceinline__ void write_dims(const TreeParams& p, long long at, const float (&o)[kN],
+                                           float f) {
+  if constexpr (kF32) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i)
+      dst[i] = make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f);
+  } else {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+#pragma unroll
+    for (int i = 0; i < kN / 8; ++i)
+      dst[i] = make_uint4(pack_bf16x2(o[8 * i] * f, o[8 * i + 1] * f),
+                          pack_bf16x2(o[8 * i + 2] * f, o[8 * i + 3] * f),
+                          pack_bf16x2(o[8 * i + 4] * f, o[8 * i + 5] * f),
+                          pack_bf16x2(o[8 * i + 6] * f, o[8 * i + 7] * f));
+  }
+}
+
+// Merges the partials of a unit that CTAs c0..c1 share, in CTA order: a lane
+// per row, the eight softmax warps split the dims (and the rows, 32 each).
+template <bool kF32>
+__device__ __forceinline__ void merge_parts(const TreeParams& p, const Segment& seg, int c0,
+                                            int c1) {
+  const int lane = threadIdx.x & 31, w = ((int)threadIdx.x >> 5) - 4;  // 0..7
+  const int rows = min(seg.info.n * p.G - seg.row_tile * kRows, kRows);
+  const int quads = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int r = (w % quads) * 32 + lane;
+  const int dims = kD * quads / 8, d0 = (w / quads) * dims;
+  if (r >= rows) return;
+  auto at = [&](int i) { return p.part + ((long long)i * 2 + (i == c0)) * kTreePartFloats; };
+  const int row = seg.row_tile * kRows + r;
+  const long long io = ((long long)(seg.info.node0 + row / p.G) * p.Hq +
+                        (long long)seg.head * p.G + row % p.G) * kD;
+  float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+  for (int i = c0; i <= c1; ++i) M = fmaxf(M, __ldcg(at(i) + kD * kRows + r));
+#pragma unroll 4
+  for (int i = c0; i <= c1; ++i) {
+    const float mi = __ldcg(at(i) + kD * kRows + r);
+    const float f = mi == -INFINITY ? 1.0f : fast_exp2(mi - M);
+    L = fmaf(__ldcg(at(i) + kD * kRows + kRows + r), f, L);
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll 1
+  for (int d = d0; d < d0 + dims; d += 16) {
+    float o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+#pragma unroll 4
+    for (int k = c0; k <= c1; ++k) {
+      const float* src = at(k);
+      const float mk = __ldcg(src + kD * kRows + r);
+      const float f = mk == -INFINITY ? 1.0f : fast_exp2(mk - M);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = fmaf(__ldcg(src + (d + i) * kRows + r), f, o[i]);
+    }
+    write_dims<kF32, 16>(p, io + d, o, inv);
+  }
 }
 
 // kF32: f32 queries and outputs (three terms each), else bf16 (one and two).
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_decode_kernel(const __grid_constant__ CUtensorMap tm_k,
-                       const __grid_constant__ CUtensorMap tm_v, TreeParams p) {
+                       const __grid_constant__ CUtensorMap tm_v,
+                       const __grid_constant__ CUtensorMap tm_q, TreeParams p) {
+  constexpr int kT = kTile, kTileBytes = kT * kD * 2;
+  constexpr int kHalfBytes = kTileBytes / 2;  // one box: kT tokens x 64 dims
   constexpr int kQ = kF32 ? 3 : 1, kP = kF32 ? 3 : 2;
-  static_assert(64 * kQ <= kColO && 32 * kP <= kColsS && kTile <= kColsS, "TMEM columns");
+  constexpr int kQBufs = kF32 ? 1 : 2;
+  constexpr int kQBytes = kQBufs * kQ * kQTermBytes;
+  constexpr int kSlots = (kOperandBytes - kQBytes) / kTileBytes;
+  static_assert(kSlots >= 4 && kSlots <= kMaxSlots, "ring");
+  // S / P buffers: four for bf16, two where P has three terms
+  constexpr int kBufs = kF32 ? 2 : 4;
+  constexpr uint32_t kColsS = 256 / kBufs;
+  static_assert(kT + (kP - 2) * kT / 2 <= (int)kColsS, "TMEM columns");
   extern __shared__ uint8_t smem_raw[];
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = sm.operands + kQBytes;
+  auto ring_slot = [](int idx) { return idx % kSlots; };
+  auto ring_parity = [](int idx) { return (uint32_t)(idx / kSlots) & 1u; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 1);
     }
-    mbar_init(&sm.q_ready, 4);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], kF32 ? 8 : 1);
+      mbar_init(&sm.q_empty[i], 1);
+      for (int k = 0; k < 4; ++k) sm.bad[i][k] = 0;
+    }
+    for (int i = 0; i < kBufs; ++i) {
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_full[i], 4);
-      mbar_init(&sm.o_done[i], 1);
-      sm.bad[i][0] = sm.bad[i][1] = 0;
     }
+    mbar_init(&sm.o_done, 1);
     sm.abort_flag = 0;
     sm.skip = timeout_recorded(p.status);
     fence_barrier_init();
@@ -200,34 +303,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(&sm.tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  const tilesplit::Run run = tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, [&](int s) {
-    const SeqInfo i = seq_info(p, s, false);
-    return tilesplit::SeqTiles{p.Hkv * row_tiles(p, i.n), key_tiles(i.ctx) + kUnitCost};
-  });
+  Walker walk;
+  walk.start(p, tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, kMinRunKeys / kT, [&](int s) {
+               const SeqInfo i = seq_info(p, s, false);
+               return tilesplit::SeqTiles{p.Hkv * row_tiles(p, i.n),
+                                          key_tiles(i.ctx) + Walker::kUnitCost};
+             }));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   volatile int* abort_flag = &sm.abort_flag;
-  Walker walk;
-  walk.start(p, run);
   if (sm.skip) walk.at = walk.end;
   Segment seg;
-  int g = 0;  // tiles of the run before the segment
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
+  if (warp < 4) {
+    regs_dec<kControlRegs>();
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- producer
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
       const uint64_t policy = l2_policy_evict_first(), keep = l2_policy_evict_last();
-      while (walk.next(p, seg)) {
+      int g = 0;
+      for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
+        if constexpr (!kF32) {
+          const int b = n_seg & 1;
+          if (n_seg >= 2)
+            mbar_wait(&sm.q_empty[b], ((n_seg >> 1) - 1) & 1, p.status, abort_flag, 114);
+          uint8_t* dst = sm.operands + b * kQTermBytes;
+          const int node = seg.info.node0 + seg.row_tile * (kRows / p.G);
+          mbar_arrive_expect_tx(&sm.q_full[b], kQTermBytes);
+          tma_load_3d(dst, &tm_q, &sm.q_full[b], 0, seg.head * p.G, node);
+          tma_load_3d(dst + kQTermBytes / 2, &tm_q, &sm.q_full[b], 64, seg.head * p.G, node);
+        }
         // keys that another row tile reads again stay in L2
         const uint64_t pol = row_tiles(p, seg.info.n) > 1 ? keep : policy;
         int block = -1;
         long long bid = 0;
         for (int j = seg.j0; j < seg.j1; ++j, ++g) {
-          const int tok = j * kTile;
+          const int tok = j * kT;
           if (tok / p.block_size != block) {
             block = tok / p.block_size;
             bid = p.block_tables[(long long)seg.seq * p.max_blocks + block];
@@ -244,73 +358,103 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (idx >= kSlots)
               mbar_wait(&sm.empty[slot], ring_parity(idx) ^ 1u, p.status, abort_flag, 103);
             const CUtensorMap* map = kv ? &tm_v : &tm_k;
-            mbar_arrive_expect_tx(&sm.full[slot], 2 * kHalfBytes);
-            tma_load_3d_hint(sm.kv[slot][0], map, &sm.full[slot], 0, seg.head, row, pol);
-            tma_load_3d_hint(sm.kv[slot][1], map, &sm.full[slot], 64, seg.head, row, pol);
+            uint8_t* dst = ring + slot * kTileBytes;
+            mbar_arrive_expect_tx(&sm.full[slot], kTileBytes);
+            tma_load_3d_hint(dst, map, &sm.full[slot], 0, seg.head, row, pol);
+            tma_load_3d_hint(dst + kHalfBytes, map, &sm.full[slot], 64, seg.head, row, pol);
           }
         }
       }
-      // Drain: the last load of every slot has landed before the CTA exits.
+      // Drain: the last load of every slot has landed before the CTA exits
+      // (the query loads precede them, and the MMAs have waited for those).
       for (int idx = max(0, 2 * g - kSlots); idx < 2 * g; ++idx)
         mbar_wait(&sm.full[ring_slot(idx)], ring_parity(idx), p.status, 104);
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kRows, kTile, 0, 0);
-      constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kRows, kD, 0, 1);
-      int n_seg = 0;
-      while (walk.next(p, seg)) {
-        mbar_wait(&sm.q_ready, n_seg & 1, p.status, abort_flag, 105);
-        ++n_seg;
-        const int n = seg.j1 - seg.j0;
-        auto issue_s = [&](int gj) {
-          const int slot = ring_slot(2 * gj);
-          mbar_wait(&sm.full[slot], ring_parity(2 * gj), p.status, abort_flag, 106);
+    // ------------------------------------------------------------ MMA issuers
+    // (each warp runs converged, so that descriptors and loop values stay
+    // warp-uniform, and elects a lane at each tcgen05 instruction: issued from
+    // a one-lane branch an MMA took ~125 cycles, so ~50)
+    auto commit = [](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+    };
+    if (warp == 1) {
+      constexpr uint32_t idesc = umma_idesc_bf16_f32(kRows, kT, 0, 0);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(sm.operands), 16, 1024);
+      const uint64_t k_desc = umma_desc_sw128(smem_u32(ring), 16, 1024);
+      int g = 0;
+      for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
+        const int n = seg.j1 - seg.j0, qb = n_seg % kQBufs;
+        mbar_wait(&sm.q_full[qb], (n_seg / kQBufs) & 1, p.status, abort_flag, 105);
+        const uint64_t qd = q_desc + (uint64_t)(qb * (kQTermBytes / 16));
+        for (int j = 0; j < n; ++j, ++g) {
+          const int slot = ring_slot(2 * g);
+          mbar_wait(&sm.full[slot], ring_parity(2 * g), p.status, abort_flag, 106);
+          if (g >= kBufs) {  // P V of the buffer's last tile is complete
+            const int idx = 2 * (g - kBufs) + 1;
+            mbar_wait(&sm.empty[ring_slot(idx)], ring_parity(idx), p.status, abort_flag, 115);
+          }
           tc_fence_after();
-          const uint32_t d = tmem + kColS + (gj & 1) * kColsS;
+          const uint64_t kd = k_desc + (uint64_t)(slot * (kTileBytes / 16));
+          const uint32_t d = tmem + kColS + (g % kBufs) * kColsS;
 #pragma unroll
           for (int t = kQ - 1; t >= 0; --t)  // the small terms first
 #pragma unroll
             for (int k = 0; k < kD / 16; ++k)
-              umma_bf16_ts(d, tmem + t * 64 + k * 8,
-                           umma_desc_sw128(smem_u32(sm.kv[slot][k >> 2]) + (k & 3) * 32, 16, 1024),
-                           idesc_s, (t < kQ - 1 || k > 0) ? 1u : 0u);
-          umma_commit(&sm.s_full[gj & 1]);
-          umma_commit(&sm.empty[slot]);
-        };
-        issue_s(g);
-        for (int j = 0; j < n; ++j) {
-          const int gj = g + j;
-          if (j + 1 < n) issue_s(gj + 1);
-          const int slot = ring_slot(2 * gj + 1);
-          mbar_wait(&sm.p_full[gj & 1], (gj >> 1) & 1, p.status, abort_flag, 107);
-          mbar_wait(&sm.full[slot], ring_parity(2 * gj + 1), p.status, abort_flag, 108);
+              if (elect_one())
+                umma_bf16(d,
+                          qd + (uint64_t)((t * kQTermBytes + (k >> 2) * (kQTermBytes / 2) +
+                                           (k & 3) * 32) / 16),
+                          kd + (uint64_t)(((k >> 2) * kHalfBytes + (k & 3) * 32) / 16), idesc,
+                          (t < kQ - 1 || k > 0) ? 1u : 0u);
+          commit(&sm.s_full[g % kBufs]);
+          commit(&sm.empty[slot]);
+        }
+        commit(&sm.q_empty[qb]);
+      }
+    } else if (warp == 2) {
+      constexpr uint32_t idesc = umma_idesc_bf16_f32(kRows, kD, 0, 1);
+      const uint64_t v_desc = umma_desc_sw128(smem_u32(ring), kHalfBytes, 1024);
+      int g = 0, n_seg = 0;
+      for (; walk.next(p, seg); ++n_seg) {
+        const int n = seg.j1 - seg.j0;
+        for (int j = 0; j < n; ++j, ++g) {
+          const int slot = ring_slot(2 * g + 1);
+          mbar_wait(&sm.p_full[g % kBufs], (g / kBufs) & 1, p.status, abort_flag, 107);
+          mbar_wait(&sm.full[slot], ring_parity(2 * g + 1), p.status, abort_flag, 108);
           tc_fence_after();
-          const uint32_t a = tmem + kColS + (gj & 1) * kColsS;
-          const uint32_t v = smem_u32(sm.kv[slot][0]);
+          const uint32_t a = tmem + kColS + (g % kBufs) * kColsS;
+          const uint64_t vd = v_desc + (uint64_t)(slot * (kTileBytes / 16));
 #pragma unroll
           for (int t = kP - 1; t >= 0; --t)
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              umma_bf16_ts(tmem + kColO, a + t * 32 + k * 8,
-                           umma_desc_sw128(v + (uint32_t)k * 16 * 128, kHalfBytes, 1024), idesc_o,
-                           (j > 0 || t < kP - 1 || k > 0) ? 1u : 0u);
-          umma_commit(&sm.o_done[gj & 1]);
-          umma_commit(&sm.empty[slot]);
+            for (int k = 0; k < kT / 16; ++k)
+              if (elect_one())
+                umma_bf16_ts(tmem + (g & 1) * kD,
+                             a + (t < 2 ? 32 * (k >> 1) + 16 * t + 8 * (k & 1) : kT + 8 * k),
+                             vd + (uint64_t)(k * 16 * 128 / 16), idesc,
+                             (j > 1 || t < kP - 1 || k > 0) ? 1u : 0u);
+          commit(&sm.empty[slot]);
         }
-        g += n;
+        commit(&sm.o_done);
       }
-      // Drain: every MMA has completed before TMEM is released.
-      if (g > 0) mbar_wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, p.status, 109);
+      // Drain: every MMA has completed before TMEM is released (each S has
+      // been waited for by the softmax before its P V).
+      if (n_seg > 0) mbar_wait(&sm.o_done, (n_seg - 1) & 1, p.status, 109);
     }
   } else {
     // ------------------------------------------------------------ softmax
+    regs_inc<kSoftmaxRegs>();
+    const int grp = (warp - 4) >> 2;  // group
+    const int tid = (int)threadIdx.x & (kGroup - 1);
     const int quad = warp & 3;  // TMEM lanes [32 * quad, 32 * quad + 32)
     const int r = quad * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const int tid = (int)threadIdx.x - 64;
-    while (walk.next(p, seg)) {
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t o_col = lanes + grp * kD;
+    const uint64_t c2 = pack2(p.scale_log2, p.scale_log2);
+    int g = 0;  // tiles of the run before the segment
+    Segment shared0, shared1;  // units shared with other CTAs: at most the run's ends
+    int n_shared = 0;
+    for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
       const int n_rows = seg.info.n * p.G;
       const int row = seg.row_tile * kRows + r;
       const bool real = row < n_rows;
@@ -319,258 +463,273 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long long io =
           ((long long)node * p.Hq + (long long)seg.head * p.G + (real ? row % p.G : 0)) * kD;
       const int first = seg.info.ctx - seg.info.n;  // position of the sequence's first node
-      // ---- queries into TMEM (the unit's S before are complete: they were
-      // waited for by the softmax that read them) ----
-      if (warp_real) {
+      if constexpr (kF32) {
+        // ---- query operand: this thread's row, dims [64 grp, 64 grp + 64)
+        // (the MMAs that read the last one are complete: o_done) ----
+        if (warp_real) {
+          uint8_t* q_row = sm.operands + grp * (kQTermBytes / 2) + r * 128;
+          const float4* src =
+              reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + io + 64 * grp);
+          float4 v[16];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if constexpr (kF32) {
-            float x[64];
-            const float4* src =
-                reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + io + 64 * hf);
+          for (int i = 0; i < 16; ++i)
+            v[i] = real ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float4 v = real ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
-            }
-#pragma unroll
-            for (int t = 0; t < kQ; ++t) {
-              uint32_t w[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) split_term(x[2 * i], x[2 * i + 1], w[i]);
-              tmem_st32(tmem + lane_off + t * 64 + hf * 32, w);
-            }
-          } else {
-            uint32_t w[32];
-            const uint4* src =
-                reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + io + 64 * hf);
+          for (int t = 0; t < kQ; ++t)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const uint4 v = real ? src[i] : make_uint4(0, 0, 0, 0);
-              w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+              uint4 w;
+              split_term(v[2 * i].x, v[2 * i].y, w.x);
+              split_term(v[2 * i].z, v[2 * i].w, w.y);
+              split_term(v[2 * i + 1].x, v[2 * i + 1].y, w.z);
+              split_term(v[2 * i + 1].z, v[2 * i + 1].w, w.w);
+              *reinterpret_cast<uint4*>(q_row + t * kQTermBytes + ((i ^ (r & 7)) << 4)) = w;
             }
-            tmem_st32(tmem + lane_off + hf * 32, w);
-          }
+          fence_proxy_async_smem();
         }
-        tmem_wait_st();
-        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[0]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_ready);
 
       float m = -INFINITY, l = 0.0f;
       const int n = seg.j1 - seg.j0;
-      for (int j = 0; j < n; ++j) {
+      const int j_first = (grp ^ g) & 1;  // the group's first tile of the segment
+      for (int j = j_first; j < n; j += 2) {
         const int gj = g + j;
-        const int col0 = (seg.j0 + j) * kTile;
-        // Which of the tile's 64 keys the row attends.
-        const bool special = col0 + kTile > first;  // holds nodes (or keys past the end)
-        uint64_t allowed = ~0ull;
-        if (special) {
-          const int rel = col0 - first;  // the first key's place among the nodes
-          uint64_t window = 0;
-          if (real) {
-            const uint64_t* words = p.mask + (long long)node * p.mask_words;
-            if (rel < 0) {
-              window = (words[0] << -rel) | ((1ull << -rel) - 1);
-            } else {
-              const int q = rel >> 6, sh = rel & 63;
-              if (q < p.mask_words) window = words[q] >> sh;
-              if (sh > 0 && q + 1 < p.mask_words) window |= words[q + 1] << (64 - sh);
-            }
-          }
-          const int here = seg.info.ctx - col0;  // keys of the context from here on, >= 1
-          allowed = here < kTile ? window & ((1ull << here) - 1) : window;
-        }
-        mbar_wait(&sm.s_full[gj & 1], (gj >> 1) & 1, p.status, abort_flag, 110);
+        const int col0 = (seg.j0 + j) * kT;
+        const uint32_t s_col = lanes + kColS + (gj % kBufs) * kColsS;
+        mbar_wait(&sm.s_full[gj % kBufs], (gj / kBufs) & 1, p.status, abort_flag, 110);
         tc_fence_after();
-        const uint32_t s_col = tmem + lane_off + kColS + (gj & 1) * kColsS;
-        float x[64];
-        if (warp_real) {
-          uint32_t w[32];
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            tmem_ld32(s_col + 32 * hf, w);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[32 * hf + i] = __uint_as_float(w[i]);
-          }
-        }
+        const bool special = col0 + kT > first;  // the tile holds nodes (or keys past the end)
+        uint64_t allowed[kT / 64];               // which of its keys the row attends
         if (special) {
+#pragma unroll
+          for (int h = 0; h < kT / 64; ++h) {
+            const int rel = col0 + 64 * h - first;  // the first key's place among the nodes
+            uint64_t w = 0;
+            if (rel <= -64) {
+              w = ~0ull;
+            } else if (real) {
+              const uint64_t* words = p.mask + (long long)node * p.mask_words;
+              if (rel < 0) {
+                w = (words[0] << -rel) | ((1ull << -rel) - 1);
+              } else {
+                const int q = rel >> 6, sh = rel & 63;
+                if (q < p.mask_words) w = words[q] >> sh;
+                if (sh > 0 && q + 1 < p.mask_words) w |= words[q + 1] << (64 - sh);
+              }
+            }
+            const int here = seg.info.ctx - col0 - 64 * h;  // keys of the context from here on
+            if (here < 64) w = here > 0 ? w & ((1ull << here) - 1) : 0;
+            allowed[h] = w;
+          }
           // V rows of nodes that hold a NaN or an infinity: 0 * NaN would
           // reach the rows whose masks leave the node out.  Such a row is
           // zeroed and noted, and makes the rows that attend it NaN.  Slots
           // past the context may hold anything and are zeroed.
           const int vidx = 2 * gj + 1, slot = ring_slot(vidx);
           mbar_wait(&sm.full[slot], ring_parity(vidx), p.status, abort_flag, 111);
-          const int t = tid >> 1;  // token of the tile; two threads, a dim half each
-          uint4* v = reinterpret_cast<uint4*>(
-              reinterpret_cast<uint8_t*>(sm.kv[slot][tid & 1]) + t * 128);
-          const bool past = col0 + t >= seg.info.ctx;
-          bool bad = false;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint4 c = v[i];
-            const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+          for (int i = 0; i < kT / 64; ++i) {
+            const int t = (tid >> 1) + 64 * i;  // key of the tile; two threads, a dim half each
+            uint4* v = reinterpret_cast<uint4*>(ring + slot * kTileBytes + (tid & 1) * kHalfBytes +
+                                                t * 128);
+            const bool past = col0 + t >= seg.info.ctx;
+            bool bad = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              bad = bad || (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
-          }
-          const uint32_t votes =
-              __ballot_sync(0xffffffffu, bad && !past && col0 + t >= first);
-          bad = (votes >> (lane & ~1)) & 3u;
-          if (bad && (tid & 1) == 0) atomicOr(&sm.bad[gj & 1][t >> 5], 1u << (t & 31));
-          if (bad || past) {
+            for (int k = 0; k < 8; ++k) {
+              const uint4 c = v[k];
+              const uint32_t u[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          named_barrier_sync(1, 128);
-          const uint64_t bad_keys = (uint64_t)sm.bad[gj & 1][1] << 32 | sm.bad[gj & 1][0];
-          if (bad_keys & allowed) l = __uint_as_float(0x7fc00000u);
-          named_barrier_sync(1, 128);
-          // (set again two tiles on at the earliest, whose S follows this P)
-          if (tid < 2) sm.bad[gj & 1][tid] = 0;
+              for (int e = 0; e < 4; ++e)
+                bad = bad || (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
+            }
+            const uint32_t votes = __ballot_sync(0xffffffffu, bad && !past && col0 + t >= first);
+            bad = (votes >> (lane & ~1)) & 3u;
+            if (bad && (tid & 1) == 0) atomicOr(&sm.bad[grp][t >> 5], 1u << (t & 31));
+            if (bad || past) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] = (allowed >> i) & 1 ? x[i] : -INFINITY;
-        }
-        if (warp_real) {
-          float top = fmaxf(x[0], x[1]);
-#pragma unroll
-          for (int i = 2; i < 64; i += 2) top = fmax3(top, x[i], x[i + 1]);
-          top *= p.scale_log2;
-          const float m_new = top > m + kSlack ? top : m;
-          const bool grows = m_new != m;
-          if (__any_sync(0xffffffffu, grows)) {
-            const float alpha = grows ? fast_exp2(m - m_new) : 1.0f;  // m = -inf: 0
-            l *= alpha;
-            m = m_new;
-            if (j > 0) {
-              // P V(j - 1) has finished: O is stable
-              mbar_wait(&sm.o_done[(gj - 1) & 1], ((gj - 1) >> 1) & 1, p.status, abort_flag, 112);
-              tc_fence_after();
-              uint32_t w[32];
-#pragma unroll
-              for (int c = 0; c < kD; c += 32) {
-                tmem_ld32(tmem + lane_off + kColO + c, w);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
-                tmem_st32(tmem + lane_off + kColO + c, w);
-              }
-              tmem_wait_st();
+              for (int k = 0; k < 8; ++k) v[k] = make_uint4(0, 0, 0, 0);
             }
           }
-          const float ref = m == -INFINITY ? 0.0f : m;  // a row without keys yet: weights 0
-          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          fence_proxy_async_smem();
+          named_barrier_sync(1 + grp, kGroup);
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            x[i] = fast_exp2(fmaf(x[i], p.scale_log2, -ref));
-            s[i & 3] += x[i];
+          for (int h = 0; h < kT / 64; ++h) {
+            const uint64_t bad_keys = (uint64_t)sm.bad[grp][2 * h + 1] << 32 | sm.bad[grp][2 * h];
+            if (bad_keys & allowed[h]) l = __uint_as_float(0x7fc00000u);
           }
-          l += (s[0] + s[1]) + (s[2] + s[3]);
+          named_barrier_sync(1 + grp, kGroup);
+          // (set again in the group's next tile, whose S follows this P)
+          if (tid < 4) sm.bad[grp][tid] = 0;
+        }
+        if (warp_real) {
+          // 32 columns at a time: scores, maximum, weights, the terms of P over
+          // the scores.
+          uint64_t s2[2] = {0, 0};
 #pragma unroll
-          for (int t = 0; t < kP; ++t) {
-            uint32_t w[32];
+          for (int c = 0; c < kT; c += 32) {
+            float x[32];
+            tmem_ld32(s_col + c, *reinterpret_cast<uint32_t(*)[32]>(&x));
+            tmem_wait_ld();
+            if (special) {
+              const uint32_t bits = (uint32_t)(allowed[c >> 6] >> (c & 63));
 #pragma unroll
-            for (int i = 0; i < 32; ++i) split_term(x[2 * i], x[2 * i + 1], w[i]);
-            tmem_st32(s_col + 32 * t, w);
+              for (int i = 0; i < 32; ++i) x[i] = (bits >> i) & 1 ? x[i] : -INFINITY;
+            }
+            float tops[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int i = 4; i < 32; i += 4)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) tops[e] = fmaxf(tops[e], x[i + e]);
+            const float top =
+                fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
+            if (__any_sync(0xffffffffu, top > m + kSlack)) {
+              // (the first columns of a unit, hardly ever again)  A new
+              // reference, a whole number, so that what is rescaled -- the
+              // sums, O_w and this tile's P so far -- changes by an exact
+              // power of two.
+              const float m_new = top > m + kSlack ? ceilf(top) : m;
+              const float up = m_new - m;  // m = -inf: infinite
+              const float alpha = up < 126.0f ? __int_as_float((127 - (int)up) << 23) : 0.0f;
+              const uint64_t a2 = pack2(alpha, alpha);
+              m = m_new;
+              l *= alpha;
+              s2[0] = fmul2(s2[0], a2);
+              s2[1] = fmul2(s2[1], a2);
+              if (j > j_first) {
+                // P V(j - 2), the group's last, must be complete: its V is free
+                const int idx = 2 * (gj - 2) + 1;
+                mbar_wait(&sm.empty[ring_slot(idx)], ring_parity(idx), p.status, abort_flag, 112);
+                tc_fence_after();
+#pragma unroll 1
+                for (int d = 0; d < kD; d += 16) {
+                  uint32_t w[16];
+                  tmem_ld16(o_col + d, w);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                    w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
+                  tmem_st16(o_col + d, w);
+                }
+              }
+#pragma unroll 1
+              for (int d = 0; d < c; d += 32)
+#pragma unroll 1
+                for (int t = 0; t < kP; ++t) {
+                  const uint32_t at = s_col + (t < 2 ? d + 16 * t : kT + d / 2);
+                  uint32_t w[16];
+                  tmem_wait_st();
+                  tmem_ld16(at, w);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                    w[i] = cvt_bf16x2(bf16lo_to_f32(w[i]) * alpha, bf16hi_to_f32(w[i]) * alpha);
+                  tmem_st16(at, w);
+                }
+              tmem_wait_st();
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;  // a row without keys yet: weights 0
+            const uint64_t r2 = pack2(-ref, -ref);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, b;
+              unpack2(ffma2(pack2(x[2 * i], x[2 * i + 1]), c2, r2), a, b);
+              x[2 * i] = fast_exp2(a);
+              x[2 * i + 1] = fast_exp2(b);
+              s2[i & 1] = fadd2(s2[i & 1], pack2(x[2 * i], x[2 * i + 1]));
+            }
+#pragma unroll
+            for (int t = 0; t < kP; ++t) {
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) split_term(x[2 * i], x[2 * i + 1], w[i]);
+              tmem_st16(s_col + (t < 2 ? c + 16 * t : kT + c / 2), w);
+            }
           }
+          float s0, s1, s3, s4;
+          unpack2(s2[0], s0, s1);
+          unpack2(s2[1], s3, s4);
+          l += (s0 + s1) + (s3 + s4);
           tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[gj & 1]);
+        if (lane == 0) mbar_arrive(&sm.p_full[gj % kBufs]);
       }
       g += n;
 
-      // ---- epilogue ----
-      mbar_wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, p.status, abort_flag, 113);
+      // ---- the unit's end: each group combines O_0 and O_1 for half of the dims ----
+      sm.m[grp][r] = m;
+      sm.l[grp][r] = l;
+      mbar_wait(&sm.o_done, n_seg & 1, p.status, abort_flag, 113);
       tc_fence_after();
+      named_barrier_sync(3, 2 * kGroup);
       const bool whole = seg.j0 == 0 && seg.j1 == seg.n_tiles;
-      auto write = [&](int c, const float (&o)[32], float f) {  // dims [c, c + 32)
-        if constexpr (kF32) {
-          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + io + c);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f,
-                                 o[4 * i + 3] * f);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + io + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[i] = make_uint4(pack_bf16x2(o[8 * i] * f, o[8 * i + 1] * f),
-                                pack_bf16x2(o[8 * i + 2] * f, o[8 * i + 3] * f),
-                                pack_bf16x2(o[8 * i + 4] * f, o[8 * i + 5] * f),
-                                pack_bf16x2(o[8 * i + 6] * f, o[8 * i + 7] * f));
-        }
-      };
       float* part = p.part + ((long long)blockIdx.x * 2 + (seg.j0 == 0 ? 1 : 0)) * kTreePartFloats;
       if (warp_real) {
-        const float f = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+        const float m0 = sm.m[0][r], m1 = sm.m[1][r];
+        const float M = fmaxf(m0, m1);
+        const float f0 = m0 == -INFINITY ? 1.0f : fast_exp2(m0 - M);
+        const float f1 = m1 == -INFINITY ? 1.0f : fast_exp2(m1 - M);
+        const float L = fmaf(sm.l[1][r], f1, sm.l[0][r] * f0);
+        const float inv = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;  // no key: zeros
+        // a segment of one tile has written only one of the two
+        const bool has0 = n > 1 || ((g - 1) & 1) == 0, has1 = n > 1 || ((g - 1) & 1) == 1;
 #pragma unroll 1
-        for (int c = 0; c < kD; c += 32) {
-          uint32_t w[32];
-          tmem_ld32(tmem + lane_off + kColO + c, w);
-          tmem_wait_ld();
+        for (int c = 64 * grp; c < 64 * grp + 64; c += 32) {
           float o[32];
+          uint32_t w0[32], w1[32];
+          if (has0) tmem_ld32(lanes + c, w0);
+          if (has1) tmem_ld32(lanes + kD + c, w1);
+          tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(w[i]);
+          for (int i = 0; i < 32; ++i)
+            o[i] = (has0 ? __uint_as_float(w0[i]) * f0 : 0.0f) +
+                   (has1 ? __uint_as_float(w1[i]) * f1 : 0.0f);
           if (whole) {
-            if (real) write(c, o, f);
+            if (real) write_dims<kF32, 32>(p, io + c, o, inv);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) part[(c + i) * kRows + r] = o[i];
           }
         }
-        if (!whole) {
-          part[kD * kRows + r] = m;
-          part[kD * kRows + kRows + r] = l;
+        if (!whole && grp == 0) {
+          part[kD * kRows + r] = M;
+          part[kD * kRows + kRows + r] = L;
         }
       }
       tc_fence_before();  // O has been read before the next unit's first P V
-      if (!whole) {
-        const int c0 = (int)(seg.unit0 / walk.per);
-        const int c1 = (int)((seg.unit0 + seg.n_tiles - 1) / walk.per);
+      if (!whole) (n_shared++ == 0 ? shared0 : shared1) = seg;
+    }
+    // ---- publish the partials; merge the units whose last one this is ----
+    if (n_shared > 0) {
+      __threadfence();
+      named_barrier_sync(3, 2 * kGroup);
+      auto ctas = [&](const Segment& u, int& c0, int& c1) {
+        c0 = (int)(u.unit0 / walk.per);
+        c1 = (int)((u.unit0 + u.n_tiles - 1) / walk.per);
+      };
+      int a0, a1, b0 = 0, b1 = 0;
+      ctas(shared0, a0, a1);
+      if (n_shared > 1) ctas(shared1, b0, b1);
+      if (tid < n_shared && grp == 0) {
+        const int c0 = tid == 0 ? a0 : b0, c1 = tid == 0 ? a1 : b1;
+        const int last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+        if (last) atomicExch(p.tickets + c0, 0);  // re-armed for the next launch
+        sm.last[tid] = last;
+      }
+      named_barrier_sync(3, 2 * kGroup);
+      if (sm.last[0]) {
         __threadfence();
-        named_barrier_sync(1, 128);
-        if (tid == 0) {
-          const int last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
-          if (last) atomicExch(p.tickets + c0, 0);  // re-armed for the next launch
-          sm.last = last;
-        }
-        named_barrier_sync(1, 128);
-        const bool last = sm.last;
-        named_barrier_sync(1, 128);
-        if (last && warp_real) {
-          __threadfence();
-          auto at = [&](int i) { return p.part + ((long long)i * 2 + (i == c0)) * kTreePartFloats; };
-          float M = -INFINITY, L = 0.0f;
-          for (int i = c0; i <= c1; ++i) M = fmaxf(M, __ldcg(at(i) + kD * kRows + r));
-          for (int i = c0; i <= c1; ++i) {
-            const float mi = __ldcg(at(i) + kD * kRows + r);
-            const float f = mi == -INFINITY ? 1.0f : fast_exp2(mi - M);
-            L = fmaf(__ldcg(at(i) + kD * kRows + kRows + r), f, L);
-          }
-          const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll 1
-          for (int c = 0; c < kD; c += 32) {
-            float o[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-            for (int k = c0; k <= c1; ++k) {
-              const float* src = at(k);
-              const float mk = __ldcg(src + kD * kRows + r);
-              const float f = mk == -INFINITY ? 1.0f : fast_exp2(mk - M);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = fmaf(__ldcg(src + (c + i) * kRows + r), f, o[i]);
-            }
-            if (real) write(c, o, inv);
-          }
-        }
+        merge_parts<kF32>(p, shared0, a0, a1);
+      }
+      if (n_shared > 1 && sm.last[1]) {
+        __threadfence();
+        merge_parts<kF32>(p, shared1, b0, b1);
       }
     }
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -582,8 +741,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <bool kF32>
-nvattn_status launch(const CUtensorMap& tk, const CUtensorMap& tv, const TreeParams& p, int grid,
-                     cudaStream_t stream) {
+nvattn_status launch(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq,
+                     const TreeParams& p, int grid, cudaStream_t stream) {
   const size_t smem = sizeof(TreeSmem) + 1024;
   // (atomic: handles on different threads may launch at the same time)
   static std::atomic<unsigned long long> attr_set_mask{0};
@@ -595,7 +754,7 @@ nvattn_status launch(const CUtensorMap& tk, const CUtensorMap& tv, const TreePar
       return NVATTN_ERR_CUDA;
     if (dev < 64) attr_set_mask.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  tree_decode_kernel<kF32><<<grid, kThreads, smem, stream>>>(tk, tv, p);
+  tree_decode_kernel<kF32><<<grid, kThreads, smem, stream>>>(tk, tv, tq, p);
   return cudaGetLastError() == cudaSuccess ? NVATTN_OK : NVATTN_ERR_CUDA;
 }
 
@@ -609,12 +768,21 @@ nvattn_status launch_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, 
                                        const int32_t* context_lens, int max_context_len,
                                        void* out, cudaStream_t stream) {
   if (n_seqs == 0 || n_nodes == 0) return NVATTN_OK;
-  CUtensorMap tk, tv;
-  nvattn_status st =
-      get_cache_tensor_map(h, k_cache, 64, kTile, CU_TENSOR_MAP_SWIZZLE_128B, &tk);
+  const bool bf16 = dtype == NVATTN_DTYPE_BF16;
+  CUtensorMap tk, tv, tq = {};
+  nvattn_status st = get_cache_tensor_map(h, k_cache, 64, kTile, CU_TENSOR_MAP_SWIZZLE_128B, &tk);
   if (st != NVATTN_OK) return st;
   st = get_cache_tensor_map(h, v_cache, 64, kTile, CU_TENSOR_MAP_SWIZZLE_128B, &tv);
   if (st != NVATTN_OK) return st;
+  if (bf16) {
+    // a unit's 128 query rows: G heads of 128 / G nodes (rows past the batch
+    // read as zeros; those of a later sequence are computed and not written)
+    const uint64_t Hq = (uint64_t)h->cfg.n_q_heads;
+    const int G = h->cfg.n_q_heads / h->cfg.n_kv_heads;
+    st = encode_tensor_map_3d(&tq, q, kD, Hq, (uint64_t)n_nodes, kD * 2, Hq * kD * 2, 64,
+                              (uint32_t)G, (uint32_t)(kRows / G), CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st != NVATTN_OK) return st;
+  }
   TreeParams p = {};
   p.Hq = h->cfg.n_q_heads;
   p.Hkv = h->cfg.n_kv_heads;
@@ -639,8 +807,8 @@ nvattn_status launch_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, 
   p.part = h->ws_part;
   p.tickets = h->part_tickets;
   p.status = h->status_dev;
-  return dtype == NVATTN_DTYPE_BF16 ? launch<false>(tk, tv, p, h->sm_count, stream)
-                                    : launch<true>(tk, tv, p, h->sm_count, stream);
+  return bf16 ? launch<false>(tk, tv, tq, p, h->sm_count, stream)
+              : launch<true>(tk, tv, tq, p, h->sm_count, stream);
 }
 
 }  // namespace nvattn
