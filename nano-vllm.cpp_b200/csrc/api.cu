@@ -71,6 +71,8 @@ nvattn_status encode_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t 
 }
 
 namespace {
+constexpr int kMapCache = 0, kMapCacheTile = 1, kMapQ8 = 2;  // NvattnTensorMapEntry::kind
+
 // Adds an entry to the handle's descriptor cache, round-robin once it is full.
 void keep_tensor_map(nvattn_handle* h, const NvattnTensorMapEntry& e) {
   int slot;
@@ -88,7 +90,7 @@ nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d
                                    int swizzle, CUtensorMap* out) {
   for (int i = 0; i < h->n_maps; ++i) {
     const NvattnTensorMapEntry& e = h->maps[i];
-    if (!e.q8 && e.base == base && e.box_d == box_d && e.box_rows == box_rows && e.swizzle == swizzle) {
+    if (e.kind == kMapCache && e.base == base && e.box_d == box_d && e.box_rows == box_rows && e.swizzle == swizzle) {
       *out = e.map;
       return NVATTN_OK;
     }
@@ -109,11 +111,40 @@ nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d
   return NVATTN_OK;
 }
 
+nvattn_status get_cache_tile_map(nvattn_handle* h, const void* base, int box_rows,
+                                 CUtensorMap* out) {
+  for (int i = 0; i < h->n_maps; ++i) {
+    const NvattnTensorMapEntry& e = h->maps[i];
+    if (e.kind == kMapCacheTile && e.base == base && e.box_rows == box_rows) {
+      *out = e.map;
+      return NVATTN_OK;
+    }
+  }
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return NVATTN_ERR_CUDA;
+  NvattnTensorMapEntry e = {};
+  e.base = base;
+  e.box_rows = box_rows;
+  e.kind = kMapCacheTile;
+  const cuuint64_t D = (cuuint64_t)h->cfg.head_dim, Hkv = (cuuint64_t)h->cfg.n_kv_heads;
+  const cuuint64_t dims[4] = {D / 2, Hkv, (cuuint64_t)h->cfg.n_layer * (cuuint64_t)h->n_slots, 2};
+  const cuuint64_t strides[3] = {D * 2, Hkv * D * 2, D};
+  const cuuint32_t box[4] = {(cuuint32_t)(D / 2), 1, (cuuint32_t)box_rows, 2};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  if (fn(&e.map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return NVATTN_ERR_CUDA;
+  keep_tensor_map(h, e);
+  *out = e.map;
+  return NVATTN_OK;
+}
+
 nvattn_status get_q8_tensor_map(nvattn_handle* h, const void* base, int box_rows,
                                 CUtensorMap* out) {
   for (int i = 0; i < h->n_maps; ++i) {
     const NvattnTensorMapEntry& e = h->maps[i];
-    if (e.q8 && e.base == base && e.box_rows == box_rows) {
+    if (e.kind == kMapQ8 && e.base == base && e.box_rows == box_rows) {
       *out = e.map;
       return NVATTN_OK;
     }
@@ -121,7 +152,7 @@ nvattn_status get_q8_tensor_map(nvattn_handle* h, const void* base, int box_rows
   NvattnTensorMapEntry e = {};
   e.base = base;
   e.box_rows = box_rows;
-  e.q8 = true;
+  e.kind = kMapQ8;
   const uint64_t D = (uint64_t)h->cfg.head_dim;
   const uint64_t page_rows = (uint64_t)h->cfg.n_kv_heads * (uint64_t)h->cfg.block_size;
   nvattn_status st = encode_tensor_map_3d(

@@ -23,7 +23,7 @@ struct NvattnTensorMapEntry {
   int box_d;     // inner box extent (elements)
   int box_rows;  // tokens per box
   int swizzle;   // CUtensorMapSwizzle value
-  bool q8;       // 8-bit pages (get_q8_tensor_map) instead of a bf16 cache
+  int kind;      // which of the get_*_tensor_map functions made it
   CUtensorMap map;
 };
 
@@ -98,6 +98,12 @@ constexpr int kMaxDecodeSeqs = 65535;
 // descriptor valid whatever later lookups do to the cache.
 nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d,
                                    int box_rows, int swizzle, CUtensorMap* out);
+
+// The same over a bf16 cache with whole 128-dim rows per box, dim halves
+// outermost: dims {64, n_kv_heads, n_layer*n_slots, 2}, box {64, 1, box_rows,
+// 2}, 128-byte swizzle -- both swizzled halves of a tile in one copy.
+nvattn_status get_cache_tile_map(nvattn_handle* h, const void* base, int box_rows,
+                                 CUtensorMap* out);
 
 // Copies into *out a TMA descriptor over the K or V pages of an 8-bit cache
 // (all layers): bytes, dims {128, n_kv_heads * block_size, n_layer *

@@ -38,10 +38,11 @@ template <class Shape>
 __device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, int min_run,
                                         Shape shape) {
   const int lane = threadIdx.x & 31;
-  long long sum = 0;
+  long long sum = 0, kept = 0;  // kept: the lane's last sequence's places
   for (int s = lane; s < n_seqs; s += 32) {
     const SeqTiles t = shape(s);
-    sum += (long long)t.units * t.tiles;
+    kept = (long long)t.units * t.tiles;
+    sum += kept;
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -57,10 +58,13 @@ __device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, int min
   }
   long long before = 0;
   for (int base = 0; base < n_seqs; base += 32) {
-    long long mine = 0;
-    if (base + lane < n_seqs) {
-      const SeqTiles t = shape(base + lane);
-      mine = (long long)t.units * t.tiles;
+    long long mine = kept;  // (one sequence per lane: nothing to read again)
+    if (n_seqs > 32) {
+      mine = 0;
+      if (base + lane < n_seqs) {
+        const SeqTiles t = shape(base + lane);
+        mine = (long long)t.units * t.tiles;
+      }
     }
     long long incl = mine;
 #pragma unroll

@@ -14,9 +14,9 @@
 // that this makes are published at the CTA's end, and the CTA that publishes a
 // unit's last one merges them, in CTA order.
 //
-//   warp 0      TMA producer: K and V tiles (two boxes of 64 dims, 128-byte
-//               swizzle) through a ring of slots that runs on across units,
-//               and before a unit's first K tile its bf16 queries (box: 64
+//   warp 0      TMA producer: K and V tiles (one copy each, the dim halves one
+//               after the other, 128-byte swizzle) through a ring of slots
+//               that runs on across units, and before a unit's first K tile its bf16 queries (box: 64
 //               dims x G heads x 128 / G nodes, the operand's layout) into one
 //               of two buffers.
 //   warp 1      TMEM allocation; issues S(j) = Q K^T (M = 128 rows, N = kTile
@@ -72,10 +72,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 32.0f;
 // A unit's end costs about as much as this many keys, and the split counts
 // them.
-constexpr int kUnitCostKeys = 256;
+constexpr int kUnitCostKeys = 512;
 // Fewest keys per CTA: below that a CTA's own start and the merge of more
 // partials cost more than the tiles.
-constexpr int kMinRunKeys = 512;
+constexpr int kMinRunKeys = 128;
 
 struct TreeParams {
   int Hq, Hkv, G, layer, block_size, max_blocks, n_seqs, n_nodes, max_nodes, mask_words;
@@ -357,11 +357,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int idx = 2 * g + kv, slot = ring_slot(idx);
             if (idx >= kSlots)
               mbar_wait(&sm.empty[slot], ring_parity(idx) ^ 1u, p.status, abort_flag, 103);
-            const CUtensorMap* map = kv ? &tm_v : &tm_k;
-            uint8_t* dst = ring + slot * kTileBytes;
             mbar_arrive_expect_tx(&sm.full[slot], kTileBytes);
-            tma_load_3d_hint(dst, map, &sm.full[slot], 0, seg.head, row, pol);
-            tma_load_3d_hint(dst + kHalfBytes, map, &sm.full[slot], 64, seg.head, row, pol);
+            tma_load_4d_hint(ring + slot * kTileBytes, kv ? &tm_v : &tm_k, &sm.full[slot], 0,
+                             seg.head, row, 0, pol);
           }
         }
       }
@@ -770,9 +768,9 @@ nvattn_status launch_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, 
   if (n_seqs == 0 || n_nodes == 0) return NVATTN_OK;
   const bool bf16 = dtype == NVATTN_DTYPE_BF16;
   CUtensorMap tk, tv, tq = {};
-  nvattn_status st = get_cache_tensor_map(h, k_cache, 64, kTile, CU_TENSOR_MAP_SWIZZLE_128B, &tk);
+  nvattn_status st = get_cache_tile_map(h, k_cache, kTile, &tk);
   if (st != NVATTN_OK) return st;
-  st = get_cache_tensor_map(h, v_cache, 64, kTile, CU_TENSOR_MAP_SWIZZLE_128B, &tv);
+  st = get_cache_tile_map(h, v_cache, kTile, &tv);
   if (st != NVATTN_OK) return st;
   if (bf16) {
     // a unit's 128 query rows: G heads of 128 / G nodes (rows past the batch

@@ -250,6 +250,7 @@ def test_bad_metadata_is_reported(cuda):
     c = tree_case(11, 16, 8, [300, 100, 400], [9, 5, 20])
     h, good = verify(c, True)
     a, b = c["cu"][1], c["cu"][2]
+    want, tol = expect(c, torch.from_numpy(c["q"]).bfloat16().float().numpy(), True)
     for field, value in (("lens", 4), ("lens", 401), ("lens", -1)):
         d = dict(c, lens=c["lens"].copy())
         d["lens"][1] = value
@@ -260,7 +261,9 @@ def test_bad_metadata_is_reported(cuda):
         assert h.get_error() == (nvattn.ERR_OUT_OF_RANGE, value)
         got = out.float().cpu().numpy()
         assert (got[a:b] == 7).all()
-        assert np.array_equal(got[:a], good[:a]) and np.array_equal(got[b:], good[b:])
+        # (the batch is split elsewhere without the skipped sequence)
+        rest = np.r_[0:a, b:len(got)]
+        Q.check(got[rest], want[rest], tol[rest], True)
     for cu in ([0, 9, 8, 34], [0, 9, 14, 35], [-1, 9, 14, 34], [0, 9, 31, 34]):
         d = dict(c, cu=np.array(cu, np.int32))
         run(d, True, h, max_nodes=20)
