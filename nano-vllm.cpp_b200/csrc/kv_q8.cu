@@ -7,7 +7,9 @@
 //
 // Bound by memory: per row 132 bytes in, 128 elements out.  Eight lanes own a
 // row (16 payload bytes each, so a row leaves as whole 32-byte sectors), and
-// each lane has kUnroll independent rows in flight; blockIdx.y is K or V.
+// each lane has kUnroll independent rows in flight (65,536 tokens x 8 kv heads
+// to bf16: 71.8 us with two, 5.7 TB/s, 89 % of the measured copy rate; 77.9 us
+// with one, 74.2 with four, 88.6 with eight); blockIdx.y is K or V.
 #include "common.cuh"
 #include "internal.h"
 
@@ -16,7 +18,7 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 2;
 constexpr int kRowsPerPass = kThreads / 8;
 
 struct LoadParams {

@@ -600,8 +600,11 @@ nvattn_status launch_store(nvattn_handle* h, KvStoreParams p, nvattn_dtype q_out
   // Large batches: bulk-copy staging (at least four stages per CTA so the
   // ring pipelines).  Small batches: the register-row kernel, which spreads
   // a few thousand rows over every SM.
-  const StagedPlan plan = plan_staged(n_tokens, p.Hq, p.Hkv);
-  if (plan.n_stages >= 3 && plan.n_chunks >= 4 * h->sm_count) {
+  // (A stage holds at least one token, so fewer tokens than that never stage;
+  // the plan's search costs a small call about a microsecond of host time.)
+  const bool many = n_tokens >= 4 * h->sm_count;
+  const StagedPlan plan = many ? plan_staged(n_tokens, p.Hq, p.Hkv) : StagedPlan{};
+  if (many && plan.n_stages >= 3 && plan.n_chunks >= 4 * h->sm_count) {
     p.rows_per_group = 0;
     switch (q_kind) {
       case kQOutBf16: return launch_staged<kQOutBf16, kQ8>(p, plan, h->sm_count, stream);

@@ -17,7 +17,7 @@
 // whose maxima come first (each of those k tiles holds at least one id that
 // precedes every id of any other tile), so the finish ranks the maxima,
 // rereads k tiles (from L2) and ranks the few logits that reach the k-th
-// maximum.  With few tiles, or more such logits than kMaxCandidates (sorted
+// maximum.  With fewer than k tiles, or more such logits than kMaxCandidates (sorted
 // logits), that limit is the k-th largest of kThreads interleaved subsets'
 // maxima; what is still too many (ties) is taken one after another.
 //
@@ -45,7 +45,7 @@ constexpr int kTile = 1024;
 constexpr int kMaxTiles = kLogprobsMaxVocab / kTile;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxCandidates = 1024;
-static_assert(kThreads <= kMaxCandidates && kMaxTop <= kThreads, "subsets");
+static_assert(kMaxTop <= kThreads, "subsets");
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -71,7 +71,7 @@ struct Smem {
   Sums part[kMaxCluster];        // CTA 0: the CTAs' sums
   Sums warp[kWarps];
   int tile[kMaxTop];             // the chosen tiles
-  uint32_t key[kMaxCandidates];  // (also the subsets' maxima)
+  uint32_t key[kMaxCandidates];
   int id[kMaxCandidates];
   uint64_t best[kWarps];
   uint32_t floor_key;
@@ -85,8 +85,23 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+constexpr uint32_t kMinusInfinity = 0x007fffffu;  // ordered(-infinity), the least key
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+// How many of the n keys (n rounded up to a multiple of 4 and zero there) come
+// before `mine` at place i: larger ones, and equal ones at a lower place.
+__device__ __forceinline__ int rank_of(const uint32_t* keys, int n, uint32_t mine, int i) {
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(keys + j);
+    rank += (o.x > mine || (o.x == mine && j < i)) + (o.y > mine || (o.y == mine && j + 1 < i)) +
+            (o.z > mine || (o.z == mine && j + 2 < i)) +
+            (o.w > mine || (o.w == mine && j + 3 < i));
+  }
+  return rank;
 }
 
 template <bool kBf16>
@@ -167,15 +182,22 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
 
   const int token = a.tokens != nullptr ? a.tokens[row_i] : -1;
   const bool has_token = token >= 0 && token < a.n_vocab;
-  const float xt = has_token ? fmaxf(load1<kBf16>(a, row, token), -INFINITY) : INFINITY;
+  float raw_xt = __uint_as_float(0x7fc00000u), xt = INFINITY;  // the token's logit; NaN as -inf
   const uint32_t keys0 = smem_peer(sm.tile_key, 0);
   if (n_ctas > 1) cluster_sync();  // CTA 0 has started: its shared memory may be written
 
   // ---- the pass ----
   Sums r = {-INFINITY, 0.0f, 0.0f, 0};
-  for (int tile = cta * kWarps + warp; tile < n_tiles; tile += n_ctas * kWarps) {
+  const int tile0 = cta * kWarps + warp;
+  for (int tile = tile0; tile < n_tiles || tile == tile0; tile += n_ctas * kWarps) {
     float x[32];
-    load_tile<kBf16, kVec>(a, row, tile, lane, x);
+    if (tile < n_tiles) load_tile<kBf16, kVec>(a, row, tile, lane, x);
+    if (tile == tile0 && has_token) {
+      // behind the first tile's loads, which do not wait for the token
+      raw_xt = load1<kBf16>(a, row, token);
+      xt = fmaxf(raw_xt, -INFINITY);
+    }
+    if (tile >= n_tiles) break;
     float top = x[0];
 #pragma unroll
     for (int e = 1; e + 1 < 32; e += 2) top = fmax3(top, x[e], x[e + 1]);
@@ -257,8 +279,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
     if (a.entropy != nullptr) a.entropy[row_i] = log_s - w.t / w.s;
     if (a.tokens != nullptr) {
       if (!has_token) record_error(a.status, NVATTN_ERR_OUT_OF_RANGE, 95, row_i);
-      const float x = has_token ? load1<kBf16>(a, row, token) : __uint_as_float(0x7fc00000u);
-      if (a.logprobs != nullptr) a.logprobs[row_i] = x - m - log_s;
+      if (a.logprobs != nullptr) a.logprobs[row_i] = raw_xt - m - log_s;
       if (a.ranks != nullptr) a.ranks[row_i] = has_token ? w.before : -1;
     }
   }
@@ -272,15 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
   __syncthreads();
   for (int i = threadIdx.x; i < n_tiles; i += kThreads) {
     const uint32_t mine = sm.tile_key[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n_tiles; j += 4) {
-      const uint4 o = *reinterpret_cast<const uint4*>(&sm.tile_key[j]);
-      // (an equal maximum counts where its tile comes first)
-      rank += (o.x > mine || (o.x == mine && j < i)) + (o.y > mine || (o.y == mine && j + 1 < i)) +
-              (o.z > mine || (o.z == mine && j + 2 < i)) +
-              (o.w > mine || (o.w == mine && j + 3 < i));
-    }
+    const int rank = rank_of(sm.tile_key, n_tiles, mine, i);
     if (rank < k_tiles) {
       sm.tile[rank] = i;
       if (rank == a.top_k - 1) sm.floor_key = mine;
@@ -289,47 +302,55 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
   __syncthreads();
 
   // ---- their logits that reach a limit which k of them reach ----
-  // A warp rereads a tile at a time, 32 logits per lane; f(key, id) is called
-  // for each logit of the vocabulary.
-  auto reread = [&](auto f) {
+  // A warp rereads a tile at a time, 32 logits per lane.  (This part runs once
+  // per row and is kept short: its instructions come from memory.)
+  int n = kMaxCandidates + 1;
+  for (int attempt = n_tiles >= a.top_k ? 0 : 1; attempt < 2 && n > kMaxCandidates; ++attempt) {
+    if (attempt == 1) {
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int i = warp; i < k_tiles; i += kWarps) {
+        float x[32];
+        load_tile<kBf16, kVec>(a, row, sm.tile[i], lane, x);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) top = fmax3(top, x[e], x[e + 1]);
+      }
+      // the k-th largest of the threads' maxima, bit by bit
+      const uint32_t mine = ordered(top);
+      uint32_t kth = 0;
+#pragma unroll 1
+      for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1)
+        if (__syncthreads_count(mine >= (kth | bit)) >= a.top_k) kth |= bit;
+      if (threadIdx.x == 0) {
+        sm.floor_key = kth;
+        sm.count = 0;
+      }
+      __syncthreads();
+    }
+    const float floor = sm.floor_key > kMinusInfinity ? value_of(sm.floor_key) : -INFINITY;
+#pragma unroll 1
     for (int i = warp; i < k_tiles; i += kWarps) {
       const int tile = sm.tile[i];
-      float x[32];
-      load_tile<kBf16, kVec>(a, row, tile, lane, x);
+      uint32_t reach = 0;
+      {
+        float x[32];
+        load_tile<kBf16, kVec>(a, row, tile, lane, x);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int id = id_of<kBf16, kVec>(tile, lane, e);
-        if (id < a.n_vocab) f(ordered(x[e]), id);
+        for (int e = 0; e < 32; ++e)
+          reach |= (fmaxf(x[e], -INFINITY) >= floor ? 1u : 0u) << e;
       }
-    }
-  };
-  int n = kMaxCandidates + 1;
-  for (int attempt = n_tiles >= 2 * a.top_k ? 0 : 1; attempt < 2 && n > kMaxCandidates;
-       ++attempt) {
-    if (attempt == 1) {
-      uint32_t mine = 0;
-      reread([&](uint32_t key, int) { mine = max(mine, key); });
-      sm.key[threadIdx.x] = mine;
-      if (threadIdx.x == 0) sm.count = 0;
-      __syncthreads();
-      int rank = 0;
-      for (int j = 0; j < kThreads; ++j) {
-        const uint32_t other = sm.key[j];
-        rank += other > mine || (other == mine && j < (int)threadIdx.x);
-      }
-      if (rank == a.top_k - 1) sm.floor_key = max(mine, 1u);
-      __syncthreads();
-    }
-    const uint32_t floor_key = max(sm.floor_key, 1u);
-    reread([&](uint32_t key, int id) {
-      if (key >= floor_key) {
-        const int at = atomicAdd(&sm.count, 1);
-        if (at < kMaxCandidates) {
-          sm.key[at] = key;
-          sm.id[at] = id;
+#pragma unroll 1
+      for (; reach != 0; reach &= reach - 1) {
+        const int id = id_of<kBf16, kVec>(tile, lane, __ffs(reach) - 1);
+        if (id < a.n_vocab) {
+          const int at = atomicAdd(&sm.count, 1);
+          if (at < kMaxCandidates) {
+            sm.key[at] = ordered(load1<kBf16>(a, row, id));
+            sm.id[at] = id;
+          }
         }
       }
-    });
+    }
     __syncthreads();
     n = sm.count;
     __syncthreads();
@@ -356,10 +377,14 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top_k; ++k) {
     uint64_t best = 0;
-    reread([&](uint32_t key, int id) {
-      const uint64_t v = (uint64_t)key << 32 | (uint32_t)~id;
-      if (v < last && v > best) best = v;
-    });
+#pragma unroll 1
+    for (int i = threadIdx.x; i < k_tiles * kTile; i += kThreads) {
+      const int id = sm.tile[i / kTile] * kTile + i % kTile;
+      if (id < a.n_vocab) {
+        const uint64_t v = (uint64_t)ordered(load1<kBf16>(a, row, id)) << 32 | (uint32_t)~id;
+        if (v < last && v > best) best = v;
+      }
+    }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1)
       best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)best, o));

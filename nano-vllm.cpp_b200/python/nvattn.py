@@ -188,19 +188,20 @@ def _stream_addr(stream):
     return None if stream is None else getattr(stream, "cuda_stream", stream)
 
 
-_dtypes = None
+class _Dtypes(dict):
+    """NVATTN_DTYPE_* by torch type, filled at the first use (torch is not
+    imported before); a type without one raises."""
 
-
-def _dtype(t):
-    """NVATTN_DTYPE_* of a float tensor (a type without one raises)."""
-    global _dtypes
-    if _dtypes is None:
+    def __missing__(self, key):
         import torch
-        _dtypes = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
-    d = _dtypes.get(t.dtype)
-    if d is None:
-        raise TypeError(f"unsupported type {t.dtype}")
-    return d
+        self.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16,
+                     torch.float16: DTYPE_F16})
+        if key not in self:
+            raise TypeError(f"unsupported type {key}")
+        return self[key]
+
+
+_DTYPES = _Dtypes()
 
 
 class Handle:
@@ -384,7 +385,7 @@ class Handle:
         if tree_mask.element_size() != 8 or tree_mask.shape[0] < q.shape[0]:
             raise ValueError("tree_mask holds 64-bit words, a row per node")
         st = lib().nvattn_paged_tree_decode(
-            self._h, layer, context_lens.shape[0], q.shape[0], _addr(q), _dtype(q),
+            self._h, layer, context_lens.shape[0], q.shape[0], _addr(q), _DTYPES[q.dtype],
             _addr(cu_nodes), _addr(tree_mask), tree_mask.shape[1], int(max_nodes),
             _addr(k_cache), _addr(v_cache), _addr(block_tables), block_tables.shape[1],
             _addr(context_lens), int(max_context_len), _addr(out), _stream_addr(stream))
@@ -400,7 +401,7 @@ class Handle:
         if V > 1 and logits.stride(1) != 1:
             raise ValueError("logits are not contiguous along the vocabulary")
         st = lib().nvattn_token_logprobs(
-            self._h, n, V, _addr(logits), _dtype(logits), max(logits.stride(0), V),
+            self._h, n, V, _addr(logits), _DTYPES[logits.dtype], max(logits.stride(0), V),
             _addr(tokens), _addr(logprobs), _addr(entropy), _addr(ranks),
             0 if top_ids is None else top_ids.shape[1], _addr(top_ids), _addr(top_logprobs),
             _stream_addr(stream))
@@ -415,7 +416,7 @@ class Handle:
         """nvattn_kv_store_q8: kv_store into the 8-bit cache."""
         st = lib().nvattn_kv_store_q8(
             self._h, layer, positions.shape[0], _addr(q), _addr(k), _addr(v), _addr(q_norm_w),
-            _addr(k_norm_w), _addr(positions), _addr(slots), _addr(q_out), _dtype(q_out),
+            _addr(k_norm_w), _addr(positions), _addr(slots), _addr(q_out), _DTYPES[q_out.dtype],
             _addr(k_q8), _addr(k_scale), _addr(v_q8), _addr(v_scale), _addr(k_rows),
             _addr(v_rows), _stream_addr(stream))
         if check:
@@ -430,7 +431,7 @@ class Handle:
             raise ValueError("k_out and v_out differ in type")
         st = lib().nvattn_kv_load_q8(
             self._h, layer, slots.shape[0], _addr(slots), _addr(k_q8), _addr(k_scale),
-            _addr(v_q8), _addr(v_scale), _dtype(k_out), _addr(k_out), _addr(v_out),
+            _addr(v_q8), _addr(v_scale), _DTYPES[k_out.dtype], _addr(k_out), _addr(v_out),
             _stream_addr(stream))
         if check:
             _check(st, "nvattn_kv_load_q8")
@@ -442,7 +443,7 @@ class Handle:
         if q.dtype != out.dtype:
             raise ValueError("q and out differ in type")
         st = lib().nvattn_paged_decode_q8(
-            self._h, layer, context_lens.shape[0], _addr(q), _dtype(q), _addr(k_q8),
+            self._h, layer, context_lens.shape[0], _addr(q), _DTYPES[q.dtype], _addr(k_q8),
             _addr(k_scale), _addr(v_q8), _addr(v_scale), _addr(block_tables),
             block_tables.shape[1], _addr(context_lens), int(max_context_len), _addr(out),
             _stream_addr(stream))
