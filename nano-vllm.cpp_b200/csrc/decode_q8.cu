@@ -13,11 +13,12 @@
 //
 // Bound by memory: 264 bytes per cached token and kv head against 2 * 128 * 2
 // products per query head.  The rows of one kv head are at most eight, so the
-// products run as mma.sync m16n8k16 on f16 (which holds e4m3 exactly) with the
-// query rows in rows 0-7 and their f16 remainders in rows 8-15: queries and
-// weights carry 22 bits at no extra cost, which a 128-row tcgen05 tile could
-// not use, and the 8-bit rows go from shared memory through registers without
-// the widened copy in shared memory that a tcgen05 operand would need.
+// products run transposed as mma.sync m16n8k16 on f16 (which holds e4m3
+// exactly): tokens or dims in M, the query rows in N = 8, and queries and
+// weights as an f16 value and its f16 remainder (22 bits) in two products.  A
+// 128-row tcgen05 tile could not use its rows, and the 8-bit rows go from
+// shared memory through registers without the widened copy in shared memory
+// that a tcgen05 operand would need.
 //
 // Each warp works alone: 32-token steps, K and V tiles of 4 KiB each by TMA
 // (128-byte swizzle) and their scales by bulk copies into its own ring of
@@ -27,13 +28,14 @@
 // merged in shared memory, and where CTAs share a unit the last of them to
 // finish merges their partials in CTA order (the same sums on every run).
 //
-// Which lane reads what.  Within the eight tokens of a score tile, column n of
-// the product is token (n >> 1) | (n & 1) << 2, and of the 16-byte chunks of a
-// V row lane g takes chunk (g >> 1) | (g & 1) << 2: with the swizzle that
-// makes every 16-byte shared load of a quarter warp hit 32 distinct banks.  A
-// lane's 16 bytes of K feed four products (the dimension order inside a dot
-// product is free, and the query operand uses the same order); of V, 16
-// products of one dimension each, after pairing the bytes of two tokens.
+// Which lane reads what.  Token n of a group of eight is row (n >> 1) |
+// (n & 1) << 2 of the group, and of the 16-byte chunks of a V row lane group g
+// takes chunk (g >> 1) | (g & 1) << 2: with the swizzle that makes every
+// 16-byte shared load of a quarter warp hit 32 distinct banks.  A lane's 16
+// bytes of K feed four products (the dimension order inside a dot product is
+// free, and the query operand uses the same order); of V, eight products of
+// two dimensions each, after pairing the bytes of two tokens.  The weights
+// turn from the scores' layout into an operand by movmatrix.
 #include <atomic>
 
 #include "common.cuh"
@@ -50,9 +52,19 @@ constexpr int kStep = 32;                // tokens per warp step
 constexpr int kTile = kWarps * kStep;    // tokens per CTA tile
 constexpr int kStages = 2;
 constexpr int kRows = 8;                 // query rows per unit (GQA group, padded)
+constexpr int kMergeRows = 2;            // rows the warps merge at a time
+static_assert(kWarps == 2 * kMergeRows, "a merge takes two warps per row");
 // A unit's start and end (its queries, the warps' merge, its rows or partial)
 // cost about as much as this many tiles, and the split counts them as such.
 constexpr int kUnitCost = 2;
+// Three CTAs per SM hide more of a warp's own latencies (64 sequences of 1k to
+// 16k tokens: 139 us, two: 145), two make fewer partials and merges (24 ragged
+// batches of 10 to 30 us: 3.5 % less in the mean).  Three where the batch may
+// hold so many tiles per CTA, by the host's bound of the contexts.
+constexpr int kFullGridTiles = 48;
+// Shared memory of a launch with two CTAs per SM: more than a third of an SM's,
+// so that no SM takes three while another takes one.
+constexpr int kTwoCtaSmem = 96 * 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;           // log2: rescale only past 2^8
 static_assert(128 % kStep == 0, "a step must not cross a block (block sizes are multiples of 128)");
@@ -82,7 +94,7 @@ struct __align__(1024) Q8Smem {
   float ks[kWarps][kStages][kStep];
   float vs[kWarps][kStages][kStep];
   float4 tok[kWarps][kStep];  // {score factor, log2 s_v, 1 / s_v, 0} of the step's tokens
-  float o[kWarps][kWarps][kD];  // of the rows being merged
+  float o[kWarps][kMergeRows][kD];  // of the rows being merged
   float m[kWarps][kRows], l[kWarps][kRows];
   uint64_t full[kWarps][kStages];
   int abort_flag;
@@ -95,6 +107,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Transposes an 8 x 8 matrix of 16-bit values, a row of four pairs per lane quad.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
 // hi = f16(x), lo = f16(x - hi) of two values, packed.
@@ -144,8 +163,8 @@ __device__ __forceinline__ void walk_next(const Q8Params& p, long long end, Walk
   }
 }
 
-// The query rows of (seq, head) as mma operands: rows scaled by a power of
-// two so that max|q| lies in [1, 2), hi parts in rows 0-7, remainders in 8-15.
+// The query rows of (seq, head) as mma operands: row g scaled by a power of two
+// so that max|q| lies in [1, 2); a[k] = {first pair hi, lo, second pair hi, lo}.
 // Returns the factor that undoes the scaling (of row g).
 template <bool kBf16>
 __device__ __forceinline__ float load_q(const Q8Params& p, int seq, int head, int g, int c,
@@ -201,18 +220,21 @@ __device__ __forceinline__ float load_q(const Q8Params& p, int seq, int head, in
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// Dims [4 * lane, 4 * lane + 4) of query row `row` of the unit.
-template <bool kBf16>
-__device__ __forceinline__ void write_out(const Q8Params& p, int seq, int head, int row, int lane,
-                                          const float4& o, float l) {
+// kN consecutive dims from `d` of query row `row` of the unit.
+template <bool kBf16, int kN>
+__device__ __forceinline__ void write_out(const Q8Params& p, int seq, int head, int row, int d,
+                                          const float (&o)[kN], float l) {
   const float f = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-  const float4 y = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-  const long long i = ((long long)seq * p.Hq + (long long)head * p.G + row) * kD + 4 * lane;
-  if constexpr (kBf16)
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + i) =
-        make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
-  else
-    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + i) = y;
+  const long long i = ((long long)seq * p.Hq + (long long)head * p.G + row) * kD + d;
+#pragma unroll
+  for (int e = 0; e < kN; e += 2) {
+    if constexpr (kBf16)
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + i + e) =
+          pack_bf16x2(o[e] * f, o[e + 1] * f);
+    else
+      *reinterpret_cast<float2*>(static_cast<float*>(p.out) + i + e) =
+          make_float2(o[e] * f, o[e + 1] * f);
+  }
 }
 
 __device__ __forceinline__ void fma4(float4& o, const float4& a, float f) {
@@ -260,7 +282,8 @@ __device__ __forceinline__ void merge_parts(const Q8Params& p, int seq, int head
         fma4(O, __ldcg(reinterpret_cast<const float4*>(at(i) + r * kD) + lane),
              __shfl_sync(0xffffffffu, f, i));
     }
-    write_out<kBf16>(p, seq, head, r, lane, O, L);
+    const float o[4] = {O.x, O.y, O.z, O.w};
+    write_out<kBf16>(p, seq, head, r, 4 * lane, o, L);
   }
 }
 
@@ -352,17 +375,20 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
   for (int i = 0; i < kStages && ahead.at < run.end; ++i) issue();
 
   uint32_t qa[8][4];
-  float o[16][4];
+  float o[8][4];  // [j]: dims 16 ch + 2 j (elements 0, 1: rows 2c, 2c + 1) and 2 j + 1 (2, 3)
   const int pr = (g >> 1) | ((g & 1) << 2);
 
   while (w.at < run.end) {
     // ---- one unit's part of the run ----
     const int seq = w.seq, head = w.head, first = w.tile, n_tiles = w.n_tiles, ctx = w.ctx;
     const long long unit0 = w.at - w.tile;
-    const float up = load_q<kBf16>(p, seq, head, g, c, qa);
-    float m = -INFINITY, l = 0.0f;
+    const float up_g = load_q<kBf16>(p, seq, head, g, c, qa);
+    // the lane's query rows from here on: 2c and 2c + 1
+    const float up[2] = {__shfl_sync(0xffffffffu, up_g, 8 * c),
+                         __shfl_sync(0xffffffffu, up_g, 8 * c + 4)};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
 
@@ -398,62 +424,77 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
           sm.tok[warp][lane] = f;
           __syncwarp();
         }
-        // ---- scores: 4 tiles of 8 tokens, their product chains interleaved ----
-        float s[4][4];
+        // ---- scores: two tiles of 16 tokens (rows g and g + 8 of the lane) ----
+        float s[2][2][4];  // [tile][product with the queries, with their remainders]
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) s[mt][0][e] = s[mt][1][e] = 0.0f;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           uint32_t u[4][4];
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt) {
-            const uint4 v = *reinterpret_cast<const uint4*>(kt + (8 * nt + pr) * kD +
+          for (int t = 0; t < 4; ++t) {
+            const uint4 v = *reinterpret_cast<const uint4*>(kt + (8 * t + pr) * kD +
                                                             (((c + 4 * hf) ^ pr) << 4));
-            u[nt][0] = v.x; u[nt][1] = v.y; u[nt][2] = v.z; u[nt][3] = v.w;
+            u[t][0] = v.x; u[t][1] = v.y; u[t][2] = v.z; u[t][3] = v.w;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
-              mma_f16(s[nt], qa[4 * hf + i], e4m3x2_to_f16x2(u[nt][i] & 0xffffu),
-                      e4m3x2_to_f16x2(u[nt][i] >> 16));
+            for (int mt = 0; mt < 2; ++mt) {
+              const uint32_t a[4] = {e4m3x2_to_f16x2(u[2 * mt][i] & 0xffffu),
+                                     e4m3x2_to_f16x2(u[2 * mt + 1][i] & 0xffffu),
+                                     e4m3x2_to_f16x2(u[2 * mt][i] >> 16),
+                                     e4m3x2_to_f16x2(u[2 * mt + 1][i] >> 16)};
+              const uint32_t(&q)[4] = qa[4 * hf + i];
+              mma_f16(s[mt][0], a, q[0], q[2]);
+              mma_f16(s[mt][1], a, q[1], q[3]);
+            }
         }
-        float x[4][2], inv[4][2];
+        float x[4][2], inv[4];  // [eight tokens][query row]
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const float4 f0 = sm.tok[warp][8 * nt + c], f1 = sm.tok[warp][8 * nt + c + 4];
-          x[nt][0] = fmaf((s[nt][0] + s[nt][2]) * up, f0.x, f0.y);
-          x[nt][1] = fmaf((s[nt][1] + s[nt][3]) * up, f1.x, f1.y);
-          inv[nt][0] = f0.z;
-          inv[nt][1] = f1.z;
+        for (int t = 0; t < 4; ++t) {
+          const float4 f = sm.tok[warp][8 * t + pr];
+          const int mt = t >> 1, e = 2 * (t & 1);
+          x[t][0] = fmaf((s[mt][0][e] + s[mt][1][e]) * up[0], f.x, f.y);
+          x[t][1] = fmaf((s[mt][0][e + 1] + s[mt][1][e + 1]) * up[1], f.x, f.y);
+          inv[t] = f.z;
         }
-        float mx = fmax3(fmax3(x[0][0], x[0][1], x[1][0]), fmax3(x[1][1], x[2][0], x[2][1]),
-                         fmaxf(x[3][0], x[3][1]));
-        if (__any_sync(0xffffffffu, mx > m + kSlack)) {
+        float top[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) top[r] = fmax3(x[0][r], x[1][r], fmaxf(x[2][r], x[3][r]));
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
           // (rare after the first step: the reference moves in strides of 2^8)
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = mx > m + kSlack ? mx : m;
-          const float alpha = m_new == m ? 1.0f : fast_exp2(m - m_new);
-          m = m_new;
-          l *= alpha;
+          float alpha[2];
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
+          for (int r = 0; r < 2; ++r) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] *= alpha;
+            for (int lanes = 4; lanes < 32; lanes *= 2)
+              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], lanes));
+            const float m_new = top[r] > m[r] + kSlack ? top[r] : m[r];
+            alpha[r] = m_new == m[r] ? 1.0f : fast_exp2(m[r] - m_new);
+            m[r] = m_new;
+            l[r] *= alpha[r];
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e & 1];
         }
-        uint32_t wa[2][4];
+        uint32_t wb[4][2];  // [eight tokens][weights, their remainders], as operands
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
+        for (int t = 0; t < 4; ++t) {
           // (a step has a key: m is -inf only where every key's score is NaN)
-          const float w0 = fast_exp2(x[nt][0] - m), w1 = fast_exp2(x[nt][1] - m);
-          l = fmaf(w0, inv[nt][0], l);
-          l = fmaf(w1, inv[nt][1], l);
-          split_f16(w0, w1, wa[nt >> 1][2 * (nt & 1)], wa[nt >> 1][2 * (nt & 1) + 1]);
+          const float w0 = fast_exp2(x[t][0] - m[0]), w1 = fast_exp2(x[t][1] - m[1]);
+          l[0] = fmaf(w0, inv[t], l[0]);
+          l[1] = fmaf(w1, inv[t], l[1]);
+          uint32_t hi, lo;
+          split_f16(w0, w1, hi, lo);
+          wb[t][0] = transpose8x8(hi);
+          wb[t][1] = transpose8x8(lo);
         }
-        // ---- o += w V8 ----
+        // ---- o += V8 w ----
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
           uint32_t v[4][4];
@@ -464,16 +505,16 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
             v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t a01 = __byte_perm(v[0][i], v[1][i], 0x5140);
-            const uint32_t a23 = __byte_perm(v[0][i], v[1][i], 0x7362);
-            const uint32_t b01 = __byte_perm(v[2][i], v[3][i], 0x5140);
-            const uint32_t b23 = __byte_perm(v[2][i], v[3][i], 0x7362);
-            mma_f16(o[4 * i], wa[ks], e4m3x2_to_f16x2(a01 & 0xffffu), e4m3x2_to_f16x2(b01 & 0xffffu));
-            mma_f16(o[4 * i + 1], wa[ks], e4m3x2_to_f16x2(a01 >> 16), e4m3x2_to_f16x2(b01 >> 16));
-            mma_f16(o[4 * i + 2], wa[ks], e4m3x2_to_f16x2(a23 & 0xffffu), e4m3x2_to_f16x2(b23 & 0xffffu));
-            mma_f16(o[4 * i + 3], wa[ks], e4m3x2_to_f16x2(a23 >> 16), e4m3x2_to_f16x2(b23 >> 16));
-          }
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t t0 = __byte_perm(v[0][i], v[1][i], h ? 0x7362 : 0x5140);
+              const uint32_t t1 = __byte_perm(v[2][i], v[3][i], h ? 0x7362 : 0x5140);
+              const uint32_t a[4] = {e4m3x2_to_f16x2(t0 & 0xffffu), e4m3x2_to_f16x2(t0 >> 16),
+                                     e4m3x2_to_f16x2(t1 & 0xffffu), e4m3x2_to_f16x2(t1 >> 16)};
+              mma_f16(o[2 * i + h], a, wb[2 * ks][0], wb[2 * ks + 1][0]);
+              mma_f16(o[2 * i + h], a, wb[2 * ks][1], wb[2 * ks + 1][1]);
+            }
         }
         __syncwarp();  // every lane has read the stage
       }
@@ -482,43 +523,48 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
       ++done;
     } while (w.at < run.end && w.tile != 0);
 
-    // ---- merge the warps: a warp per row, four dimensions per lane ----
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (c == 0) {
-      sm.m[warp][g] = m;
-      sm.l[warp][g] = l;
+    // ---- merge the warps: two warps per row, two dimensions per lane ----
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int lanes = 4; lanes < 32; lanes *= 2)
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], lanes);
+      if (g == 0) {
+        sm.m[warp][2 * c + r] = m[r];
+        sm.l[warp][2 * c + r] = l[r];
+      }
     }
     const bool whole = first == 0 && done == n_tiles;
     float* part = p.part + ((long long)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * kQ8PartFloats;
-    for (int r0 = 0; r0 < p.G; r0 += kWarps) {
-      if (g >= r0 && g < min(p.G, r0 + kWarps)) {
+    for (int r0 = 0; r0 < p.G; r0 += kMergeRows) {
+      if (2 * c == r0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float4*>(&sm.o[warp][g - r0][64 * e + 16 * c + 4 * j]) =
-                make_float4(o[4 * j][e] + o[4 * j][e + 2], o[4 * j + 1][e] + o[4 * j + 1][e + 2],
-                            o[4 * j + 2][e] + o[4 * j + 2][e + 2],
-                            o[4 * j + 3][e] + o[4 * j + 3][e + 2]);
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(&sm.o[warp][r][16 * pr + 4 * j]) = make_float4(
+                o[2 * j][r], o[2 * j][2 + r], o[2 * j + 1][r], o[2 * j + 1][2 + r]);
       }
       __syncthreads();
-      if (const int r = r0 + warp; r < p.G) {
+      const int r = r0 + (warp & 1), d = 64 * (warp >> 1) + 2 * lane;
+      if (r < p.G) {
         float M = -INFINITY, L = 0.0f;
-        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float O[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.m[i][r]);
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
           const float f = sm.m[i][r] == -INFINITY ? 1.0f : fast_exp2(sm.m[i][r] - M);
-          fma4(O, *reinterpret_cast<const float4*>(&sm.o[i][warp][4 * lane]), f);
+          const float2 v = *reinterpret_cast<const float2*>(&sm.o[i][warp & 1][d]);
+          O[0] = fmaf(v.x, f, O[0]);
+          O[1] = fmaf(v.y, f, O[1]);
           L = fmaf(sm.l[i][r], f, L);
         }
         if (whole) {
-          write_out<kBf16>(p, seq, head, r, lane, O, L);
+          write_out<kBf16>(p, seq, head, r, d, O, L);
         } else {
-          *reinterpret_cast<float4*>(part + r * kD + 4 * lane) = O;
-          if (lane == 0) {
+          *reinterpret_cast<float2*>(part + r * kD + d) = make_float2(O[0], O[1]);
+          if (d == 0) {
             part[kRows * kD + r] = M;
             part[kRows * kD + kRows + r] = L;
           }
@@ -584,7 +630,11 @@ nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, co
   p.part = h->ws_part;
   p.tickets = h->part_tickets;
   p.status = h->status_dev;
-  const size_t smem = sizeof(Q8Smem) + 1024;
+  const long long tiles = (long long)n_seqs * p.Hkv * ((max_context_len + kTile - 1) / kTile);
+  const int per_sm = tiles >= (long long)kFullGridTiles * kQ8CtasPerSm * h->sm_count
+                         ? kQ8CtasPerSm : kQ8CtasPerSm - 1;
+  const size_t smem = per_sm == kQ8CtasPerSm ? sizeof(Q8Smem) + 1024 : kTwoCtaSmem;
+  static_assert(kQ8CtasPerSm == 3 && sizeof(Q8Smem) + 1024 <= kTwoCtaSmem, "two per SM");
   static_assert(kQ8CtasPerSm * (sizeof(Q8Smem) + 2048) <= 228 * 1024, "CTAs per SM");
   // (atomic: handles on different threads may launch at the same time)
   static std::atomic<unsigned long long> attr_set_mask{0};
@@ -592,13 +642,13 @@ nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, co
   if (cudaGetDevice(&dev) != cudaSuccess) return NVATTN_ERR_CUDA;
   if (dev >= 64 || !(attr_set_mask.load(std::memory_order_relaxed) & (1ull << dev))) {
     if (cudaFuncSetAttribute(decode_q8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem) != cudaSuccess ||
+                             kTwoCtaSmem) != cudaSuccess ||
         cudaFuncSetAttribute(decode_q8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem) != cudaSuccess)
+                             kTwoCtaSmem) != cudaSuccess)
       return NVATTN_ERR_CUDA;
     if (dev < 64) attr_set_mask.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  const int grid = kQ8CtasPerSm * h->sm_count;
+  const int grid = per_sm * h->sm_count;
   if (dtype == NVATTN_DTYPE_BF16)
     decode_q8_kernel<true><<<grid, kThreads, smem, stream>>>(tk, tv, p);
   else

@@ -138,7 +138,7 @@ nvattn_status launch_kv_load_q8(nvattn_handle* h, int layer, int n_tokens, const
                                 const float* v_scale, nvattn_dtype out_dtype, void* k_out,
                                 void* v_out, cudaStream_t stream);
 constexpr int kQ8Warps = 4;
-constexpr int kQ8CtasPerSm = 2;
+constexpr int kQ8CtasPerSm = 3;
 // one partial: 8 rows of 128, then 8 references and 8 sums
 constexpr int kQ8PartFloats = 8 * 128 + 16;
 // Attention for trees of drafted tokens (tree_decode.cu), one CTA per SM; a
