@@ -21,6 +21,9 @@ ops in the reference, is not vendored).  As in ggml's mul_mat with bf16
 weights, activations are rounded to bf16, products accumulate in f32 and
 the outputs stay f32; the residual stream and the norms are f32.
 
+With kv_cache="q8" the K/V cache is the 8-bit one: each layer stores the new
+rows with nvattn_kv_store_q8 and attends with nvattn_paged_decode_q8.
+
 The attention path is a parameter (`attention`): the library by default; a
 test substitutes the CPU oracle to compare whole steps.  Block tables follow
 BlockManager::Append (block_manager.cpp:162-184): a sequence takes a new
@@ -119,11 +122,15 @@ def rms_norm(x, w, eps):
 class DecodeRunner:
     """One decode step of a batch through all layers (ModelRunner::Run,
     decode branch) with the KV cache in the reference's layout:
-    [n_layer][num_blocks * 256][n_kv_heads][head_dim] bf16, K and V."""
+    [n_layer][num_blocks * 256][n_kv_heads][head_dim] bf16, K and V; with
+    kv_cache="q8" in the 8-bit pages of nvattn_kv_store_q8 (q8_cache: K payload,
+    K scale, V payload, V scale)."""
 
     def __init__(self, shape: Qwen3Shape, weights: Qwen3Weights, num_blocks, max_seqs,
-                 max_blocks, device, attention=None):
+                 max_blocks, device, attention=None, kv_cache="bf16"):
         import torch
+        if kv_cache not in ("bf16", "q8"):
+            raise ValueError("kv_cache is \"bf16\" or \"q8\"")
         self.shape, self.w, self.device = shape, weights, device
         self.max_blocks = max_blocks
         self.max_context = max_blocks * BS
@@ -134,10 +141,18 @@ class DecodeRunner:
                                   rope_theta=shape.rope_theta, device=device.index or 0)
         self.h = nvattn.Handle(cfg)
         n_slots = num_blocks * BS
-        self.k_cache = torch.zeros((shape.n_layer, n_slots, shape.n_kv_heads, shape.head_dim),
-                                   dtype=torch.int16, device=device)
-        self.v_cache = torch.zeros_like(self.k_cache)
-        self.attention = attention or self.library_attention
+        self.k_cache = self.v_cache = self.q8_cache = None
+        if kv_cache == "q8":
+            pages = (shape.n_layer, num_blocks, shape.n_kv_heads, BS)
+            self.q8_cache = [t for _ in "kv" for t in (
+                torch.zeros(pages + (shape.head_dim,), dtype=torch.uint8, device=device),
+                torch.zeros(pages, device=device))]
+        else:
+            self.k_cache = torch.zeros((shape.n_layer, n_slots, shape.n_kv_heads, shape.head_dim),
+                                       dtype=torch.int16, device=device)
+            self.v_cache = torch.zeros_like(self.k_cache)
+        self.attention = attention or (self.library_attention if self.q8_cache is None
+                                       else self.library_attention_q8)
         # per-step device inputs (fixed addresses, so a captured step replays)
         self.bufs = None
         self.attn_events = None  # [(start, end)] per layer when timing
@@ -152,6 +167,7 @@ class DecodeRunner:
             "slots": torch.zeros(n_seqs, dtype=torch.int32, device=dev),
             "bt": torch.zeros((n_seqs, self.max_blocks), dtype=torch.int32, device=dev),
             "attn": torch.empty((n_seqs, self.shape.n_q_heads, self.shape.head_dim), device=dev),
+            "q": torch.empty((n_seqs, self.shape.n_q_heads, self.shape.head_dim), device=dev),
             "next": torch.zeros(n_seqs, dtype=torch.int32, device=dev),
             "logits": torch.empty((n_seqs, self.shape.vocab), device=dev),
             "temps": torch.zeros(n_seqs, device=dev),
@@ -172,6 +188,34 @@ class DecodeRunner:
                            self.v_cache, b["bt"], b["ctx"], self.max_context, b["attn"],
                            stream=stream)
         return b["attn"]
+
+    def library_attention_q8(self, layer, q, k, v, stream=None):
+        """The same over the 8-bit cache: the store (normed q into bufs['q']),
+        then the decode."""
+        import torch
+        stream = stream or torch.cuda.current_stream(self.device)
+        b, L = self.bufs, self.w.layers[layer]
+        self.h.kv_store_q8(layer, q, k, v, L["q_norm"], L["k_norm"], b["pos"], b["slots"], b["q"],
+                           *self.q8_cache, stream=stream)
+        self.h.decode_q8(layer, b["q"], *self.q8_cache, b["bt"], b["ctx"], self.max_context,
+                         b["attn"], stream=stream)
+        return b["attn"]
+
+    def token_logprobs(self, tokens=None, top_k=0, stream=None):
+        """Log-probabilities under the last step's logits (nvattn_token_logprobs):
+        of `tokens` (int32; default: the step's own), their ranks, the rows'
+        entropies and the top_k alternatives, as a dict of device tensors."""
+        import torch
+        b, dev = self.bufs, self.device
+        n = b["logits"].shape[0]
+        out = {"logprobs": torch.empty(n, device=dev), "entropy": torch.empty(n, device=dev),
+               "ranks": torch.empty(n, dtype=torch.int32, device=dev)}
+        if top_k:
+            out["top_ids"] = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+            out["top_logprobs"] = torch.empty((n, top_k), device=dev)
+        self.h.token_logprobs(b["logits"], b["next"] if tokens is None else tokens, **out,
+                              stream=stream or torch.cuda.current_stream(dev))
+        return out
 
     def set_inputs(self, tokens, tables: BlockTables):
         """Host side of the step: PrepareInputs' positions / slots (the new
