@@ -39,8 +39,7 @@
 // add as much error as the rounding of a bf16 output itself).  f32 queries and
 // their P are sums of three bf16 terms, 24 bits: f32 in, f32 out.
 // TMEM columns: O_0 [0, 128), O_1 [128, 256), then the S / P buffers, tile j in
-// buffer j % kBufs: P holds, over each 32 keys' own scores, their first terms
-// and their second terms (16 columns each), the third terms behind the tile's
+// buffer j % kBufs: P's terms, 32 columns each, over the tile's 64 columns of
 // scores.  With four buffers (bf16) a group finds its next scores there while
 // its last P V still runs; with two, score, softmax and P V of a group's tiles
 // follow one another.
@@ -59,8 +58,8 @@ constexpr int kTile = 64;  // keys per tile
 constexpr int kGroup = 128;  // softmax threads of one group
 constexpr int kThreads = 3 * kGroup;
 // Registers per thread: 168 at launch (384 threads); the softmax groups take
-// what warps 0-3 give up: 136 + 2 * 184 = 3 * 168.
-constexpr int kControlRegs = 136, kSoftmaxRegs = 184;
+// what warps 0-3 give up: 88 + 2 * 208 = 3 * 168.
+constexpr int kControlRegs = 88, kSoftmaxRegs = 208;
 constexpr int kQTermBytes = kRows * kD * 2;     // [d half][row][64], 128-byte swizzle
 constexpr int kOperandBytes = 13 * 16 * 1024;  // query operands and the ring share it
 constexpr uint32_t kTmemCols = 512;
@@ -92,20 +91,6 @@ struct TreeParams {
   int* tickets;  // [CTA], zero between launches
   DeviceStatus* status;
 };
-
-constexpr int kMaxSlots = 13;
-struct __align__(1024) TreeSmem {
-  uint8_t operands[kOperandBytes];  // query terms, then the K / V ring
-  uint64_t full[kMaxSlots], empty[kMaxSlots];
-  uint64_t q_full[2], q_empty[2], s_full[4], p_full[4], o_done;
-  float m[2][kRows], l[2][kRows];  // the groups' references and sums at a unit's end
-  uint32_t bad[2][4];  // [group]: keys of its tile whose V row holds a NaN or an infinity
-  uint32_t tmem_base;
-  int abort_flag;
-  int skip;
-  int last[2];
-};
-static_assert(sizeof(TreeSmem) + 1024 <= 227 * 1024, "shared memory");
 
 // A sequence's nodes and context; n = 0 where it has none or its metadata is
 // unusable (`report`: recorded then).
@@ -139,17 +124,32 @@ struct Segment {
   long long unit0;  // place of the unit's first tile
 };
 
+constexpr int kMaxSlots = 13;
+struct __align__(1024) TreeSmem {
+  uint8_t operands[kOperandBytes];  // query terms, then the K / V ring
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t q_full[2], q_empty[2], s_full[4], p_full[4], o_done;
+  float m[2][kRows], l[2][kRows];  // the groups' references and sums at a unit's end
+  uint32_t bad[2][4];  // [group]: keys of its tile whose V row holds a NaN or an infinity
+  uint32_t tmem_base;
+  int abort_flag;
+  int skip;
+  int last[2];
+  Segment shared[2];  // units shared with other CTAs: at most the run's ends
+  long long per;      // places per CTA
+};
+static_assert(sizeof(TreeSmem) + 1024 <= 227 * 1024, "shared memory");
+
 // Walks the segments of a run; every role walks the same ones.
 struct Walker {
   static constexpr int kUnitCost = kUnitCostKeys / kTile;
-  long long at, end, per;
+  long long at, end;
   int seq, unit;  // the unit that `at` lies in
   SeqInfo info;
 
   __device__ __forceinline__ void start(const TreeParams& p, const tilesplit::Run& r) {
     at = r.begin;
     end = r.end;
-    per = r.per;
     seq = r.seq;
     unit = 0;
     if (at >= end) return;
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // S / P buffers: four for bf16, two where P has three terms
   constexpr int kBufs = kF32 ? 2 : 4;
   constexpr uint32_t kColsS = 256 / kBufs;
-  static_assert(kT + (kP - 2) * kT / 2 <= (int)kColsS, "TMEM columns");
+  static_assert(kT <= (int)kColsS && kP * kT / 2 <= (int)kColsS, "TMEM columns");
   extern __shared__ uint8_t smem_raw[];
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -304,11 +304,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   Walker walk;
-  walk.start(p, tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, kMinRunKeys / kT, [&](int s) {
-               const SeqInfo i = seq_info(p, s, false);
-               return tilesplit::SeqTiles{p.Hkv * row_tiles(p, i.n),
-                                          key_tiles(i.ctx) + Walker::kUnitCost};
-             }));
+  const tilesplit::Run run =
+      tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, kMinRunKeys / kT, [&](int s) {
+        const SeqInfo i = seq_info(p, s, false);
+        return tilesplit::SeqTiles{p.Hkv * row_tiles(p, i.n), key_tiles(i.ctx) + Walker::kUnitCost};
+      });
+  walk.start(p, run);
+  if (threadIdx.x == 0) sm.per = run.per;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -323,7 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------- producer
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      const uint64_t policy = l2_policy_evict_first(), keep = l2_policy_evict_last();
+      // (evict_first also where a kv head has several row tiles, whose reads
+      // come close together: 16 ragged drafts took 109 us with it, 117 without)
+      const uint64_t policy = l2_policy_evict_first();
       int g = 0;
       for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
         if constexpr (!kF32) {
@@ -336,8 +340,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_3d(dst, &tm_q, &sm.q_full[b], 0, seg.head * p.G, node);
           tma_load_3d(dst + kQTermBytes / 2, &tm_q, &sm.q_full[b], 64, seg.head * p.G, node);
         }
-        // keys that another row tile reads again stay in L2
-        const uint64_t pol = row_tiles(p, seg.info.n) > 1 ? keep : policy;
         int block = -1;
         long long bid = 0;
         for (int j = seg.j0; j < seg.j1; ++j, ++g) {
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               mbar_wait(&sm.empty[slot], ring_parity(idx) ^ 1u, p.status, abort_flag, 103);
             mbar_arrive_expect_tx(&sm.full[slot], kTileBytes);
             tma_load_4d_hint(ring + slot * kTileBytes, kv ? &tm_v : &tm_k, &sm.full[slot], 0,
-                             seg.head, row, 0, pol);
+                             seg.head, row, 0, policy);
           }
         }
       }
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < kT / 16; ++k)
               if (elect_one())
                 umma_bf16_ts(tmem + (g & 1) * kD,
-                             a + (t < 2 ? 32 * (k >> 1) + 16 * t + 8 * (k & 1) : kT + 8 * k),
+                             a + 32 * t + 8 * k,
                              vd + (uint64_t)(k * 16 * 128 / 16), idesc,
                              (j > 1 || t < kP - 1 || k > 0) ? 1u : 0u);
           commit(&sm.empty[slot]);
@@ -450,7 +452,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_col = lanes + grp * kD;
     const uint64_t c2 = pack2(p.scale_log2, p.scale_log2);
     int g = 0;  // tiles of the run before the segment
-    Segment shared0, shared1;  // units shared with other CTAs: at most the run's ends
     int n_shared = 0;
     for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
       const int n_rows = seg.info.n * p.G;
@@ -562,88 +563,66 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (tid < 4) sm.bad[grp][tid] = 0;
         }
         if (warp_real) {
-          // 32 columns at a time: scores, maximum, weights, the terms of P over
-          // the scores.
-          uint64_t s2[2] = {0, 0};
+          float x[kT];
 #pragma unroll
-          for (int c = 0; c < kT; c += 32) {
-            float x[32];
-            tmem_ld32(s_col + c, *reinterpret_cast<uint32_t(*)[32]>(&x));
-            tmem_wait_ld();
-            if (special) {
-              const uint32_t bits = (uint32_t)(allowed[c >> 6] >> (c & 63));
+          for (int c = 0; c < kT; c += 32)
+            tmem_ld32(s_col + c, *reinterpret_cast<uint32_t(*)[32]>(&x[c]));
+          tmem_wait_ld();
+          if (special) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = (bits >> i) & 1 ? x[i] : -INFINITY;
-            }
-            float tops[4] = {x[0], x[1], x[2], x[3]};
+            for (int i = 0; i < kT; ++i)
+              x[i] = (allowed[i >> 6] >> (i & 63)) & 1 ? x[i] : -INFINITY;
+          }
+          float tops[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int i = 4; i < 32; i += 4)
+          for (int i = 4; i + 4 < kT; i += 8)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) tops[e] = fmaxf(tops[e], x[i + e]);
-            const float top =
-                fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
-            if (__any_sync(0xffffffffu, top > m + kSlack)) {
-              // (the first columns of a unit, hardly ever again)  A new
-              // reference, a whole number, so that what is rescaled -- the
-              // sums, O_w and this tile's P so far -- changes by an exact
-              // power of two.
-              const float m_new = top > m + kSlack ? ceilf(top) : m;
-              const float up = m_new - m;  // m = -inf: infinite
-              const float alpha = up < 126.0f ? __int_as_float((127 - (int)up) << 23) : 0.0f;
-              const uint64_t a2 = pack2(alpha, alpha);
-              m = m_new;
-              l *= alpha;
-              s2[0] = fmul2(s2[0], a2);
-              s2[1] = fmul2(s2[1], a2);
-              if (j > j_first) {
-                // P V(j - 2), the group's last, must be complete: its V is free
-                const int idx = 2 * (gj - 2) + 1;
-                mbar_wait(&sm.empty[ring_slot(idx)], ring_parity(idx), p.status, abort_flag, 112);
-                tc_fence_after();
+            for (int e = 0; e < 4; ++e) tops[e] = fmax3(tops[e], x[i + e], x[i + 4 + e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tops[e] = fmaxf(tops[e], x[kT - 4 + e]);
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
+          if (__any_sync(0xffffffffu, top > m + kSlack)) {
+            // (the first tile of a unit, hardly ever again)  A new reference;
+            // the sums and O_w so far are rescaled.
+            const float m_new = top > m + kSlack ? top : m;
+            const float alpha = m_new == m ? 1.0f : fast_exp2(m - m_new);  // m = -inf: 0
+            m = m_new;
+            l *= alpha;
+            if (j > j_first) {
+              // P V(j - 2), the group's last, must be complete: its V is free
+              const int idx = 2 * (gj - 2) + 1;
+              mbar_wait(&sm.empty[ring_slot(idx)], ring_parity(idx), p.status, abort_flag, 112);
+              tc_fence_after();
 #pragma unroll 1
-                for (int d = 0; d < kD; d += 16) {
-                  uint32_t w[16];
-                  tmem_ld16(o_col + d, w);
-                  tmem_wait_ld();
+              for (int d = 0; d < kD; d += 16) {
+                uint32_t w[16];
+                tmem_ld16(o_col + d, w);
+                tmem_wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 16; ++i)
-                    w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
-                  tmem_st16(o_col + d, w);
-                }
+                for (int i = 0; i < 16; ++i)
+                  w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
+                tmem_st16(o_col + d, w);
               }
-#pragma unroll 1
-              for (int d = 0; d < c; d += 32)
-#pragma unroll 1
-                for (int t = 0; t < kP; ++t) {
-                  const uint32_t at = s_col + (t < 2 ? d + 16 * t : kT + d / 2);
-                  uint32_t w[16];
-                  tmem_wait_st();
-                  tmem_ld16(at, w);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i)
-                    w[i] = cvt_bf16x2(bf16lo_to_f32(w[i]) * alpha, bf16hi_to_f32(w[i]) * alpha);
-                  tmem_st16(at, w);
-                }
               tmem_wait_st();
             }
-            const float ref = m == -INFINITY ? 0.0f : m;  // a row without keys yet: weights 0
-            const uint64_t r2 = pack2(-ref, -ref);
+          }
+          const float ref = m == -INFINITY ? 0.0f : m;  // a row without keys yet: weights 0
+          const uint64_t r2 = pack2(-ref, -ref);
+          uint64_t s2[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float a, b;
-              unpack2(ffma2(pack2(x[2 * i], x[2 * i + 1]), c2, r2), a, b);
-              x[2 * i] = fast_exp2(a);
-              x[2 * i + 1] = fast_exp2(b);
-              s2[i & 1] = fadd2(s2[i & 1], pack2(x[2 * i], x[2 * i + 1]));
-            }
+          for (int i = 0; i < kT / 2; ++i) {
+            float a, b;
+            unpack2(ffma2(pack2(x[2 * i], x[2 * i + 1]), c2, r2), a, b);
+            x[2 * i] = fast_exp2(a);
+            x[2 * i + 1] = fast_exp2(b);
+            s2[i & 1] = fadd2(s2[i & 1], pack2(x[2 * i], x[2 * i + 1]));
+          }
 #pragma unroll
-            for (int t = 0; t < kP; ++t) {
-              uint32_t w[16];
+          for (int t = 0; t < kP; ++t) {
+            uint32_t w[32];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) split_term(x[2 * i], x[2 * i + 1], w[i]);
-              tmem_st16(s_col + (t < 2 ? c + 16 * t : kT + c / 2), w);
-            }
+            for (int i = 0; i < 32; ++i) split_term(x[2 * i], x[2 * i + 1], w[i]);
+            tmem_st32(s_col + 32 * t, w);
           }
           float s0, s1, s3, s4;
           unpack2(s2[0], s0, s1);
@@ -698,34 +677,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tc_fence_before();  // O has been read before the next unit's first P V
-      if (!whole) (n_shared++ == 0 ? shared0 : shared1) = seg;
+      if (!whole) {
+        if (threadIdx.x == kGroup) sm.shared[n_shared] = seg;
+        ++n_shared;
+      }
     }
     // ---- publish the partials; merge the units whose last one this is ----
     if (n_shared > 0) {
       __threadfence();
       named_barrier_sync(3, 2 * kGroup);
       auto ctas = [&](const Segment& u, int& c0, int& c1) {
-        c0 = (int)(u.unit0 / walk.per);
-        c1 = (int)((u.unit0 + u.n_tiles - 1) / walk.per);
+        c0 = (int)(u.unit0 / sm.per);
+        c1 = (int)((u.unit0 + u.n_tiles - 1) / sm.per);
       };
-      int a0, a1, b0 = 0, b1 = 0;
-      ctas(shared0, a0, a1);
-      if (n_shared > 1) ctas(shared1, b0, b1);
+      int c0, c1;
       if (tid < n_shared && grp == 0) {
-        const int c0 = tid == 0 ? a0 : b0, c1 = tid == 0 ? a1 : b1;
+        ctas(sm.shared[tid], c0, c1);
         const int last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
         if (last) atomicExch(p.tickets + c0, 0);  // re-armed for the next launch
         sm.last[tid] = last;
       }
       named_barrier_sync(3, 2 * kGroup);
-      if (sm.last[0]) {
-        __threadfence();
-        merge_parts<kF32>(p, shared0, a0, a1);
-      }
-      if (n_shared > 1 && sm.last[1]) {
-        __threadfence();
-        merge_parts<kF32>(p, shared1, b0, b1);
-      }
+#pragma unroll 1
+      for (int i = 0; i < n_shared; ++i)
+        if (sm.last[i]) {
+          __threadfence();
+          ctas(sm.shared[i], c0, c1);
+          merge_parts<kF32>(p, sm.shared[i], c0, c1);
+        }
     }
     __syncwarp();
   }

@@ -401,7 +401,7 @@ class Handle:
         if V > 1 and logits.stride(1) != 1:
             raise ValueError("logits are not contiguous along the vocabulary")
         st = lib().nvattn_token_logprobs(
-            self._h, n, V, _addr(logits), _DTYPES[logits.dtype], max(logits.stride(0), V),
+            self._h, n, V, _addr(logits), _DTYPES[logits.dtype], logits.stride(0) if n > 1 else V,
             _addr(tokens), _addr(logprobs), _addr(entropy), _addr(ranks),
             0 if top_ids is None else top_ids.shape[1], _addr(top_ids), _addr(top_logprobs),
             _stream_addr(stream))

@@ -211,6 +211,7 @@ def test_refusals(h):
     assert go(x, t, f, top_ids=torch.zeros((2, 65), dtype=torch.int32, device="cuda"),
               top_logprobs=kf) == no
     assert go(torch.zeros((1, 2097153), device="cuda"), t, f) == no
+    assert go(x[:1].expand(2, 100), t, f) == bad  # one row for all: stride 0
     with pytest.raises(ValueError):
         go(x.t(), t, f)
     with pytest.raises(TypeError):
