@@ -10,15 +10,15 @@
 // of a kv head read its keys together: 512 bytes per token and kv head for up
 // to 128 rows, bound by memory until a kv head has several row tiles (whose
 // keys then come from L2).  The units' key tiles (kTile keys) are split evenly
-// over one CTA per SM (tile_split.cuh); the partials
-// that this makes are published at the CTA's end, and the CTA that publishes a
-// unit's last one merges them, in CTA order.
+// over one CTA per SM (tile_split.cuh); the partials that this makes are
+// published at the CTA's end, and the CTA that publishes a unit's last one
+// merges them, in CTA order.
 //
 //   warp 0      TMA producer: K and V tiles (one copy each, the dim halves one
-//               after the other, 128-byte swizzle) through a ring of slots
-//               that runs on across units, and before a unit's first K tile its bf16 queries (box: 64
-//               dims x G heads x 128 / G nodes, the operand's layout) into one
-//               of two buffers.
+//               after the other, 128-byte swizzle) through two rings of
+//               slots that run on across units, and before a unit's first K tile
+//               its bf16 queries (box: 64 dims x G heads x 128 / G nodes, the
+//               operand's layout) into one of two buffers.
 //   warp 1      TMEM allocation; issues S(j) = Q K^T (M = 128 rows, N = kTile
 //               keys), up to kBufs tiles ahead, into the next unit too, so that
 //               a unit's first scores are there when its softmax starts.
@@ -126,7 +126,7 @@ struct Segment {
 
 constexpr int kMaxSlots = 13;
 struct __align__(1024) TreeSmem {
-  uint8_t operands[kOperandBytes];  // query terms, then the K / V ring
+  uint8_t operands[kOperandBytes];  // query terms, then the K slots, then the V slots
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2], s_full[4], p_full[4], o_done;
   float m[2][kRows], l[2][kRows];  // the groups' references and sums at a unit's end
@@ -265,21 +265,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kQ = kF32 ? 3 : 1, kP = kF32 ? 3 : 2;
   constexpr int kQBufs = kF32 ? 1 : 2;
   constexpr int kQBytes = kQBufs * kQ * kQTermBytes;
-  constexpr int kSlots = (kOperandBytes - kQBytes) / kTileBytes;
-  static_assert(kSlots >= 4 && kSlots <= kMaxSlots, "ring");
   // S / P buffers: four for bf16, two where P has three terms
   constexpr int kBufs = kF32 ? 2 : 4;
+  constexpr int kSlotsK = kF32 ? 3 : 4, kSlotsV = kF32 ? 4 : 5;
+  static_assert(kQBytes + (kSlotsK + kSlotsV) * kTileBytes <= kOperandBytes &&
+                kSlotsK + kSlotsV <= kMaxSlots, "ring");
+  // P V(t) is waited for on V(t)'s `empty` barrier, by the S issuer at tile t +
+  // kBufs and by the softmax at t + 2.  The slot's next use ends with P V(t +
+  // kSlotsV), which comes after that waiter's own tile's (P Vs are issued in
+  // order), so the barrier cannot be two uses ahead of the wait.
+  static_assert(kSlotsV >= kBufs && kSlotsV >= 2, "V slots");
   constexpr uint32_t kColsS = 256 / kBufs;
   static_assert(kT <= (int)kColsS && kP * kT / 2 <= (int)kColsS, "TMEM columns");
   extern __shared__ uint8_t smem_raw[];
   TreeSmem& sm = *reinterpret_cast<TreeSmem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = sm.operands + kQBytes;
-  auto ring_slot = [](int idx) { return idx % kSlots; };
-  auto ring_parity = [](int idx) { return (uint32_t)(idx / kSlots) & 1u; };
+  // slots of tile g's K and V, and the parity of their use
+  auto k_slot = [](int g) { return g % kSlotsK; };
+  auto k_parity = [](int g) { return (uint32_t)(g / kSlotsK) & 1u; };
+  auto v_slot = [](int g) { return kSlotsK + g % kSlotsV; };
+  auto v_parity = [](int g) { return (uint32_t)(g / kSlotsV) & 1u; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) {
+    for (int i = 0; i < kSlotsK + kSlotsV; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 1);
     }
@@ -356,9 +365,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 tok % p.block_size);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            const int idx = 2 * g + kv, slot = ring_slot(idx);
-            if (idx >= kSlots)
-              mbar_wait(&sm.empty[slot], ring_parity(idx) ^ 1u, p.status, abort_flag, 103);
+            const int slot = kv ? v_slot(g) : k_slot(g);
+            if (g >= (kv ? kSlotsV : kSlotsK))
+              mbar_wait(&sm.empty[slot], (kv ? v_parity(g) : k_parity(g)) ^ 1u, p.status,
+                        abort_flag, 103);
             mbar_arrive_expect_tx(&sm.full[slot], kTileBytes);
             tma_load_4d_hint(ring + slot * kTileBytes, kv ? &tm_v : &tm_k, &sm.full[slot], 0,
                              seg.head, row, 0, policy);
@@ -367,8 +377,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // Drain: the last load of every slot has landed before the CTA exits
       // (the query loads precede them, and the MMAs have waited for those).
-      for (int idx = max(0, 2 * g - kSlots); idx < 2 * g; ++idx)
-        mbar_wait(&sm.full[ring_slot(idx)], ring_parity(idx), p.status, 104);
+      for (int i = max(0, g - kSlotsK); i < g; ++i)
+        mbar_wait(&sm.full[k_slot(i)], k_parity(i), p.status, 104);
+      for (int i = max(0, g - kSlotsV); i < g; ++i)
+        mbar_wait(&sm.full[v_slot(i)], v_parity(i), p.status, 104);
     }
     // ------------------------------------------------------------ MMA issuers
     // (each warp runs converged, so that descriptors and loop values stay
@@ -387,12 +399,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(&sm.q_full[qb], (n_seg / kQBufs) & 1, p.status, abort_flag, 105);
         const uint64_t qd = q_desc + (uint64_t)(qb * (kQTermBytes / 16));
         for (int j = 0; j < n; ++j, ++g) {
-          const int slot = ring_slot(2 * g);
-          mbar_wait(&sm.full[slot], ring_parity(2 * g), p.status, abort_flag, 106);
-          if (g >= kBufs) {  // P V of the buffer's last tile is complete
-            const int idx = 2 * (g - kBufs) + 1;
-            mbar_wait(&sm.empty[ring_slot(idx)], ring_parity(idx), p.status, abort_flag, 115);
-          }
+          const int slot = k_slot(g), prev = g - kBufs;
+          mbar_wait(&sm.full[slot], k_parity(g), p.status, abort_flag, 106);
+          if (prev >= 0)  // P V of the buffer's last tile is complete
+            mbar_wait(&sm.empty[v_slot(prev)], v_parity(prev), p.status, abort_flag, 115);
           tc_fence_after();
           const uint64_t kd = k_desc + (uint64_t)(slot * (kTileBytes / 16));
           const uint32_t d = tmem + kColS + (g % kBufs) * kColsS;
@@ -418,9 +428,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; walk.next(p, seg); ++n_seg) {
         const int n = seg.j1 - seg.j0;
         for (int j = 0; j < n; ++j, ++g) {
-          const int slot = ring_slot(2 * g + 1);
+          const int slot = v_slot(g);
           mbar_wait(&sm.p_full[g % kBufs], (g / kBufs) & 1, p.status, abort_flag, 107);
-          mbar_wait(&sm.full[slot], ring_parity(2 * g + 1), p.status, abort_flag, 108);
+          mbar_wait(&sm.full[slot], v_parity(g), p.status, abort_flag, 108);
           tc_fence_after();
           const uint32_t a = tmem + kColS + (g % kBufs) * kColsS;
           const uint64_t vd = v_desc + (uint64_t)(slot * (kTileBytes / 16));
@@ -526,8 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           // reach the rows whose masks leave the node out.  Such a row is
           // zeroed and noted, and makes the rows that attend it NaN.  Slots
           // past the context may hold anything and are zeroed.
-          const int vidx = 2 * gj + 1, slot = ring_slot(vidx);
-          mbar_wait(&sm.full[slot], ring_parity(vidx), p.status, abort_flag, 111);
+          const int slot = v_slot(gj);
+          mbar_wait(&sm.full[slot], v_parity(gj), p.status, abort_flag, 111);
 #pragma unroll
           for (int i = 0; i < kT / 64; ++i) {
             const int t = (tid >> 1) + 64 * i;  // key of the tile; two threads, a dim half each
@@ -590,8 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             l *= alpha;
             if (j > j_first) {
               // P V(j - 2), the group's last, must be complete: its V is free
-              const int idx = 2 * (gj - 2) + 1;
-              mbar_wait(&sm.empty[ring_slot(idx)], ring_parity(idx), p.status, abort_flag, 112);
+              mbar_wait(&sm.empty[v_slot(gj - 2)], v_parity(gj - 2), p.status, abort_flag, 112);
               tc_fence_after();
 #pragma unroll 1
               for (int d = 0; d < kD; d += 16) {
@@ -676,7 +685,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           part[kD * kRows + kRows + r] = L;
         }
       }
-      tc_fence_before();  // O has been read before the next unit's first P V
+      // Neither group goes on before the other has read both O, both sums and
+      // o_done: its next P would start the next unit's P V over them.
+      tc_fence_before();
+      named_barrier_sync(3, 2 * kGroup);
       if (!whole) {
         if (threadIdx.x == kGroup) sm.shared[n_shared] = seg;
         ++n_shared;

@@ -222,6 +222,39 @@ def test_deterministic_and_replayed(cuda):
     h.check_device()
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+def test_scores_that_keep_rising(cuda, bf16):
+    """Each tile's scores pass the last one's by far more than the reference's
+    slack (2^32), so every tile rescales; then the same falling."""
+    rng = np.random.default_rng(13)
+    for sign in (1, -1):
+        c = tree_case(14, 16, 8, [1500, 700], [30, 3])
+        d = rng.standard_normal(128)
+        d /= np.linalg.norm(d)
+        c["q"] = (d * 12 + 0.05 * rng.standard_normal(c["q"].shape)).astype(np.float32)
+        for s, n in enumerate(c["lens"]):
+            sl = Q.slots_of(c["bt"][s], n, 256)
+            # d.k up to n / 10: in steps of 8 sqrt(128) log2-units per 64 keys and more
+            rise = sign * np.arange(n)[:, None, None] / 10.0 * d
+            c["k"][0, sl] = O.f32_to_bf16((rise + 0.05 * rng.standard_normal(
+                (n, 8, 128))).astype(np.float32))
+        verify(c, bf16)
+
+
+def test_many_short_units_repeat_exactly(cuda):
+    """Units of one to five key tiles one after another on every CTA, again and
+    again: the hand-over between units has no room for a stale accumulator."""
+    rng = np.random.default_rng(15)
+    lens = rng.integers(1, 300, 400)
+    nodes = np.minimum(rng.integers(1, 40, 400), lens)
+    c = tree_case(16, 16, 8, lens.tolist(), nodes.tolist())
+    for bf16 in (True, False):
+        h, first = verify(c, bf16)
+        for _ in range(20):
+            assert np.array_equal(run(c, bf16, h)[1], first)
+        h.check_device()
+
+
 def test_the_8_bit_decode_shares_the_workspace(cuda):
     """Tree and 8-bit decodes alternating on one handle: both leave their
     tickets as they found them."""
