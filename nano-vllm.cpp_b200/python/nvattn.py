@@ -1,7 +1,8 @@
 """Python binding of libnvattn through its C ABI (include/nvattn.h), via ctypes.
 
 This is the ctypes stub a Python caller (tests, benchmarks) uses; tensors are
-passed as raw device pointers, so no framework type crosses the ABI.  The
+passed as raw device pointers, so no framework type crosses the ABI; they are
+contiguous tensors on the handle's device unless a method says otherwise.  The
 library is loaded from nano-vllm.cpp_b200/lib/libnvattn.so and there is no
 fallback: a missing library raises.
 """
@@ -185,7 +186,9 @@ def _addr(t):
 
 
 def _stream_addr(stream):
-    return None if stream is None else getattr(stream, "cuda_stream", stream)
+    if stream is None:
+        return None
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
 class _Dtypes(dict):
@@ -212,6 +215,7 @@ class Handle:
         h = _vp()
         _check(lib().nvattn_create(ctypes.byref(cfg), ctypes.byref(h)), "nvattn_create")
         self._h = h
+        self._L = lib()
 
     def close(self):
         if getattr(self, "_h", None):
@@ -384,11 +388,12 @@ class Handle:
             raise ValueError("q and out differ in type")
         if tree_mask.element_size() != 8 or tree_mask.shape[0] < q.shape[0]:
             raise ValueError("tree_mask holds 64-bit words, a row per node")
-        st = lib().nvattn_paged_tree_decode(
-            self._h, layer, context_lens.shape[0], q.shape[0], _addr(q), _DTYPES[q.dtype],
-            _addr(cu_nodes), _addr(tree_mask), tree_mask.shape[1], int(max_nodes),
-            _addr(k_cache), _addr(v_cache), _addr(block_tables), block_tables.shape[1],
-            _addr(context_lens), int(max_context_len), _addr(out), _stream_addr(stream))
+        st = self._L.nvattn_paged_tree_decode(
+            self._h, layer, context_lens.shape[0], q.shape[0], q.data_ptr(), _DTYPES[q.dtype],
+            cu_nodes.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], int(max_nodes),
+            k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+            block_tables.shape[1], context_lens.data_ptr(), int(max_context_len), out.data_ptr(),
+            _stream_addr(stream))
         if check:
             _check(st, "nvattn_paged_tree_decode")
         return st
@@ -400,7 +405,7 @@ class Handle:
         n, V = logits.shape
         if V > 1 and logits.stride(1) != 1:
             raise ValueError("logits are not contiguous along the vocabulary")
-        st = lib().nvattn_token_logprobs(
+        st = self._L.nvattn_token_logprobs(
             self._h, n, V, _addr(logits), _DTYPES[logits.dtype], logits.stride(0) if n > 1 else V,
             _addr(tokens), _addr(logprobs), _addr(entropy), _addr(ranks),
             0 if top_ids is None else top_ids.shape[1], _addr(top_ids), _addr(top_logprobs),
@@ -414,11 +419,12 @@ class Handle:
     def kv_store_q8(self, layer, q, k, v, q_norm_w, k_norm_w, positions, slots, q_out, k_q8,
                     k_scale, v_q8, v_scale, stream=None, check=True, k_rows=None, v_rows=None):
         """nvattn_kv_store_q8: kv_store into the 8-bit cache."""
-        st = lib().nvattn_kv_store_q8(
-            self._h, layer, positions.shape[0], _addr(q), _addr(k), _addr(v), _addr(q_norm_w),
-            _addr(k_norm_w), _addr(positions), _addr(slots), _addr(q_out), _DTYPES[q_out.dtype],
-            _addr(k_q8), _addr(k_scale), _addr(v_q8), _addr(v_scale), _addr(k_rows),
-            _addr(v_rows), _stream_addr(stream))
+        st = self._L.nvattn_kv_store_q8(
+            self._h, layer, positions.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            q_norm_w.data_ptr(), k_norm_w.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+            q_out.data_ptr(), _DTYPES[q_out.dtype], k_q8.data_ptr(), k_scale.data_ptr(),
+            v_q8.data_ptr(), v_scale.data_ptr(), _addr(k_rows), _addr(v_rows),
+            _stream_addr(stream))
         if check:
             _check(st, "nvattn_kv_store_q8")
         return st
@@ -427,12 +433,13 @@ class Handle:
                    check=True):
         """nvattn_kv_load_q8: the slots' rows into k_out / v_out
         [n_tokens][Hkv][128] (f32, bf16 or f16, the same for both)."""
-        if k_out.dtype != v_out.dtype:
+        dtype = k_out.dtype
+        if v_out.dtype != dtype:
             raise ValueError("k_out and v_out differ in type")
-        st = lib().nvattn_kv_load_q8(
-            self._h, layer, slots.shape[0], _addr(slots), _addr(k_q8), _addr(k_scale),
-            _addr(v_q8), _addr(v_scale), _DTYPES[k_out.dtype], _addr(k_out), _addr(v_out),
-            _stream_addr(stream))
+        st = self._L.nvattn_kv_load_q8(
+            self._h, layer, slots.shape[0], slots.data_ptr(), k_q8.data_ptr(), k_scale.data_ptr(),
+            v_q8.data_ptr(), v_scale.data_ptr(), _DTYPES[dtype], k_out.data_ptr(),
+            v_out.data_ptr(), _stream_addr(stream))
         if check:
             _check(st, "nvattn_kv_load_q8")
         return st
@@ -440,12 +447,13 @@ class Handle:
     def decode_q8(self, layer, q, k_q8, k_scale, v_q8, v_scale, block_tables, context_lens,
                   max_context_len, out, stream=None, check=True):
         """nvattn_paged_decode_q8: q and out f32 or bf16, the same for both."""
-        if q.dtype != out.dtype:
+        dtype = q.dtype
+        if out.dtype != dtype:
             raise ValueError("q and out differ in type")
-        st = lib().nvattn_paged_decode_q8(
-            self._h, layer, context_lens.shape[0], _addr(q), _DTYPES[q.dtype], _addr(k_q8),
-            _addr(k_scale), _addr(v_q8), _addr(v_scale), _addr(block_tables),
-            block_tables.shape[1], _addr(context_lens), int(max_context_len), _addr(out),
+        st = self._L.nvattn_paged_decode_q8(
+            self._h, layer, context_lens.shape[0], q.data_ptr(), _DTYPES[dtype], k_q8.data_ptr(),
+            k_scale.data_ptr(), v_q8.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+            block_tables.shape[1], context_lens.data_ptr(), int(max_context_len), out.data_ptr(),
             _stream_addr(stream))
         if check:
             _check(st, "nvattn_paged_decode_q8")

@@ -411,21 +411,22 @@ def test_refusals(cuda):
     with pytest.raises(ValueError):
         dec(q=q.bfloat16())
     assert dec(q=q.view(-1)[1:]) == bad  # not 16-byte aligned
-    for i in range(4):
-        assert dec(d=[None if j == i else x for j, x in enumerate(d)]) == bad
     assert dec(lens=lens[:0]) == nvattn.OK
     slots = torch.zeros(2, dtype=torch.int32, device="cuda")
     ko = torch.zeros((2, 8, 128), device="cuda")
     load = lambda slots=slots, ko=ko, vo=ko.clone(), d=d: h.kv_load_q8(  # noqa: E731
         0, slots, *d, ko, vo, check=False)
     assert load() == nvattn.OK and load(slots=slots[:0]) == nvattn.OK
-    assert load(d=[d[0], None, d[2], d[3]]) == bad
     with pytest.raises(TypeError):
         load(ko=ko.double(), vo=ko.double())
     with pytest.raises(ValueError):
         load(ko=ko.half())
     L, n = nvattn.lib(), None
     p = ctypes.c_void_p(d[0].data_ptr())
+    for i in range(4):
+        c4 = [None if j == i else p for j in range(4)]
+        assert L.nvattn_paged_decode_q8(h._h, 0, 1, p, 0, *c4, p, 2, p, 300, p, n) == bad
+        assert L.nvattn_kv_load_q8(h._h, 0, 1, p, *c4, 0, p, p, n) == bad
     assert L.nvattn_kv_store_q8(h._h, 0, 1, p, p, p, p, p, p, p, p, 0, p, p, p, p, p, n, n) == bad
     assert L.nvattn_kv_store_q8(h._h, 0, 1, p, p, p, p, p, p, p, p, 9, p, p, p, p, n, n, n) == bad
     h.check_device()

@@ -327,7 +327,12 @@ def test_refusals(cuda):
 
     assert go() == nvattn.OK
     assert go(layer=1) == bad and go(mn=65) == bad and go(mn=-1) == bad and go(mc=301) == bad
-    assert go(k=None) == bad and go(cu=None) == bad and go(bt=a["bt"][:, :1]) == bad
+    assert go(bt=a["bt"][:, :1]) == bad
+    p, L = q.data_ptr(), nvattn.lib()
+    for i in range(7):  # q, cu_nodes, mask, k, v, tables, lengths: each of them null
+        x = [None if j == i else p for j in range(7)]
+        assert L.nvattn_paged_tree_decode(h._h, 0, 2, 14, x[0], 0, x[1], x[2], 1, 9, x[3], x[4],
+                                          x[5], 2, x[6], 300, p, None) == bad
     assert go(q=q.half(), out=out.half()) == bad
     assert go(lens=torch.zeros(3, dtype=torch.int32, device="cuda")) == bad
     assert go(lens=a["lens"][:0]) == nvattn.OK and go(q=q[:0], out=out[:0]) == nvattn.OK
