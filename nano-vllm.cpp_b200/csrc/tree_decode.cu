@@ -78,7 +78,7 @@ constexpr int kMinRunKeys = 128;
 
 struct TreeParams {
   int Hq, Hkv, G, layer, block_size, max_blocks, n_seqs, n_nodes, max_nodes, mask_words;
-  int max_context;
+  int max_context, row_tiles;  // row_tiles: of a sequence of max_nodes
   long long n_slots, num_blocks;
   float scale_log2;
   const void* q;
@@ -97,6 +97,11 @@ struct TreeParams {
 struct SeqInfo {
   int node0, n, ctx;
 };
+// The units' order: row tile by row tile, each over all sequences and their kv
+// heads (entry e of the line: row tile e / n_seqs of sequence e % n_seqs).  The
+// row tiles of a kv head then lie a large part of the line apart, where other
+// CTAs read the same keys at about the same time, mostly from L2; one after
+// another they would be read by one CTA, the second time from memory.
 __device__ __forceinline__ SeqInfo seq_info(const TreeParams& p, int s, bool report) {
   const int a = p.cu_nodes[s], b = p.cu_nodes[s + 1];
   int ctx = p.context_lens[s];
@@ -110,8 +115,10 @@ __device__ __forceinline__ SeqInfo seq_info(const TreeParams& p, int s, bool rep
   }
   return {a, b - a, ctx};
 }
-__device__ __forceinline__ int row_tiles(const TreeParams& p, int n) {
-  return (n * p.G + kRows - 1) / kRows;
+__device__ __forceinline__ SeqInfo entry_info(const TreeParams& p, int e) {
+  SeqInfo i = seq_info(p, e % p.n_seqs, false);
+  if ((e / p.n_seqs) * kRows >= i.n * p.G) i.n = 0;  // no such row tile
+  return i;
 }
 __device__ __forceinline__ int key_tiles(int ctx) {
   return (ctx + kTile - 1) / kTile;
@@ -144,21 +151,20 @@ static_assert(sizeof(TreeSmem) + 1024 <= 227 * 1024, "shared memory");
 struct Walker {
   static constexpr int kUnitCost = kUnitCostKeys / kTile;
   long long at, end;
-  int seq, unit;  // the unit that `at` lies in
+  int entry, head;  // the unit that `at` lies in
+  int offset;       // place of `at` in its unit
   SeqInfo info;
 
   __device__ __forceinline__ void start(const TreeParams& p, const tilesplit::Run& r) {
     at = r.begin;
     end = r.end;
-    seq = r.seq;
-    unit = 0;
+    entry = r.seq;
     if (at >= end) return;
-    info = seq_info(p, seq, false);
+    info = entry_info(p, entry);
     const int span = key_tiles(info.ctx) + kUnitCost;
-    unit = (int)((at - r.seq_first) / span);
+    head = (int)((at - r.seq_first) / span);
     offset = (int)((at - r.seq_first) % span);
   }
-  int offset;  // place of `at` in its unit
 
   __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
     while (at < end) {
@@ -166,19 +172,16 @@ struct Walker {
       const int left = tiles + kUnitCost - offset;
       const int take = (int)min((long long)left, end - at);
       const int j0 = max(offset - kUnitCost, 0), j1 = offset + take - kUnitCost;
-      bool some = j1 > j0;
-      if (some) {
-        const int rt = row_tiles(p, info.n);
-        s = {seq, unit / rt, unit % rt, j0, j1, tiles, info, at - offset + kUnitCost};
-      }
+      const bool some = j1 > j0;
+      if (some)
+        s = {entry % p.n_seqs, head, entry / p.n_seqs, j0, j1, tiles, info,
+             at - offset + kUnitCost};
       at += take;
       offset = 0;
-      if (take == left && at < end) {
-        if (++unit == p.Hkv * row_tiles(p, info.n)) {
-          unit = 0;
-          do info = seq_info(p, ++seq, false);
-          while (info.n == 0);  // (`at` < end: a later sequence has places)
-        }
+      if (take == left && at < end && ++head == p.Hkv) {
+        head = 0;
+        do info = entry_info(p, ++entry);
+        while (info.n == 0);  // (`at` < end: a later entry has places)
       }
       if (some) return true;
     }
@@ -214,43 +217,57 @@ __device__ __forceinline__ void write_dims(const TreeParams& p, long long at, co
 
 // Merges the partials of a unit that CTAs c0..c1 share, in CTA order: a lane
 // per row, the eight softmax warps split the dims (and the rows, 32 each).
+// Four partials at a time, with all of their loads in flight together: the
+// reads are bound by their latency where the rows are few, and by what one SM
+// reads from L2 (about 110 GB/s) where they are many.
 template <bool kF32>
 __device__ __forceinline__ void merge_parts(const TreeParams& p, const Segment& seg, int c0,
                                             int c1) {
+  constexpr int kAtOnce = 4, kDims = 16;
   const int lane = threadIdx.x & 31, w = ((int)threadIdx.x >> 5) - 4;  // 0..7
   const int rows = min(seg.info.n * p.G - seg.row_tile * kRows, kRows);
   const int quads = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   const int r = (w % quads) * 32 + lane;
   const int dims = kD * quads / 8, d0 = (w / quads) * dims;
   if (r >= rows) return;
-  auto at = [&](int i) { return p.part + ((long long)i * 2 + (i == c0)) * kTreePartFloats; };
   const int row = seg.row_tile * kRows + r;
   const long long io = ((long long)(seg.info.node0 + row / p.G) * p.Hq +
                         (long long)seg.head * p.G + row % p.G) * kD;
-  float M = -INFINITY, L = 0.0f;
-#pragma unroll 4
-  for (int i = c0; i <= c1; ++i) M = fmaxf(M, __ldcg(at(i) + kD * kRows + r));
-#pragma unroll 4
-  for (int i = c0; i <= c1; ++i) {
-    const float mi = __ldcg(at(i) + kD * kRows + r);
-    const float f = mi == -INFINITY ? 1.0f : fast_exp2(mi - M);
-    L = fmaf(__ldcg(at(i) + kD * kRows + kRows + r), f, L);
-  }
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll 1
-  for (int d = d0; d < d0 + dims; d += 16) {
-    float o[16];
+  for (int d = d0; d < d0 + dims; d += kDims) {
+    float o[kDims], M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = 0.0f;
-#pragma unroll 4
-    for (int k = c0; k <= c1; ++k) {
-      const float* src = at(k);
-      const float mk = __ldcg(src + kD * kRows + r);
-      const float f = mk == -INFINITY ? 1.0f : fast_exp2(mk - M);
+    for (int i = 0; i < kDims; ++i) o[i] = 0.0f;
+#pragma unroll 1
+    for (int k = c0; k <= c1; k += kAtOnce) {
+      float v[kAtOnce][kDims], m[kAtOnce], l[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = fmaf(__ldcg(src + (d + i) * kRows + r), f, o[i]);
+      for (int e = 0; e < kAtOnce; ++e) {
+        // (the first CTA left its part in its second place: tile_split.cuh;
+        // behind the last part: that part again, with no weight)
+        const int i = min(k + e, c1);
+        const float* src = p.part + ((long long)i * 2 + (i == c0)) * kTreePartFloats + r;
+        m[e] = __ldcg(src + kD * kRows);
+        l[e] = __ldcg(src + kD * kRows + kRows);
+#pragma unroll
+        for (int j = 0; j < kDims; ++j) v[e][j] = __ldcg(src + (d + j) * kRows);
+      }
+      const float top = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), M);
+      const float old = M == -INFINITY ? 1.0f : fast_exp2(M - top);
+      M = top;
+      L *= old;
+#pragma unroll
+      for (int j = 0; j < kDims; ++j) o[j] *= old;
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        if (k + e > c1) break;
+        const float f = m[e] == -INFINITY ? 1.0f : fast_exp2(m[e] - top);
+        L = fmaf(l[e], f, L);
+#pragma unroll
+        for (int j = 0; j < kDims; ++j) o[j] = fmaf(v[e][j], f, o[j]);
+      }
     }
-    write_dims<kF32, 16>(p, io + d, o, inv);
+    write_dims<kF32, kDims>(p, io + d, o, L == 0.0f ? 0.0f : 1.0f / L);
   }
 }
 
@@ -314,10 +331,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Walker walk;
   const tilesplit::Run run =
-      tilesplit::find_run(p.n_seqs, blockIdx.x, gridDim.x, kMinRunKeys / kT, [&](int s) {
-        const SeqInfo i = seq_info(p, s, false);
-        return tilesplit::SeqTiles{p.Hkv * row_tiles(p, i.n), key_tiles(i.ctx) + Walker::kUnitCost};
-      });
+      tilesplit::find_run(p.n_seqs * p.row_tiles, blockIdx.x, gridDim.x, kMinRunKeys / kT,
+                          [&](int e) {
+                            const SeqInfo i = entry_info(p, e);
+                            return tilesplit::SeqTiles{i.n > 0 ? p.Hkv : 0,
+                                                       key_tiles(i.ctx) + Walker::kUnitCost};
+                          });
   walk.start(p, run);
   if (threadIdx.x == 0) sm.per = run.per;
   tc_fence_before();
@@ -784,6 +803,7 @@ nvattn_status launch_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, 
   p.max_nodes = max_nodes;
   p.mask_words = mask_words;
   p.max_context = max_context_len;
+  p.row_tiles = (max_nodes * p.G + kRows - 1) / kRows;
   p.n_slots = h->n_slots;
   p.num_blocks = h->cfg.num_blocks;
   p.scale_log2 = h->cfg.scale * kLog2e;
