@@ -108,7 +108,8 @@ NVATTN_API void nvattn_config_init_qwen3(nvattn_config* cfg);
 
 /* Validates cfg, builds the RoPE cos/sin table (ggml's float recurrence,
  * computed on the host once and copied to the device) and allocates the
- * split-KV workspace and status word.  Replaces the KV/backend set-up of
+ * split-KV workspace (with 20 MB of partials for nvattn_paged_decode_q8 and
+ * nvattn_paged_tree_decode) and status word.  Replaces the KV/backend set-up of
  * Qwen3Model::Qwen3Model (qwen3.cpp:99-108, 186-213), whose failures throw;
  * here they return a status. */
 NVATTN_API nvattn_status nvattn_create(const nvattn_config* cfg, nvattn_handle** out);
@@ -471,7 +472,10 @@ NVATTN_API nvattn_status nvattn_paged_prefill_rows(
  * whose cu_nodes or context_lens are unusable (N_s negative or above max_nodes,
  * rows outside n_nodes, context_lens[s] outside [N_s, max_context_len]) is
  * reported as NVATTN_ERR_OUT_OF_RANGE and its rows are not written.
- * The launch uses the handle's workspace: calls on one handle are issued on
+ * NVATTN_ERR_UNSUPPORTED for batches whose bounds allow 2^30 key tiles (64
+ * keys each, counted per kv head and 128 query rows) or more.
+ * Results repeat bit for bit for a batch; another batch composition splits a
+ * context elsewhere and may move the last bits.  The launch uses the handle's workspace: calls on one handle are issued on
  * one stream, as for nvattn_paged_decode. */
 NVATTN_API nvattn_status nvattn_paged_tree_decode(
     nvattn_handle* h, int layer, int n_seqs, int n_nodes, const void* q_dev, nvattn_dtype dtype,
@@ -525,6 +529,9 @@ NVATTN_API nvattn_status nvattn_kv_load_q8(
  * [n_seqs][n_q_heads][head_dim] in dtype, f32 or bf16 (sums in f32 either
  * way; queries and softmax weights carry 22 bits).  Slots behind a sequence's
  * context may hold anything.  A sequence of length 0 gives zeros.
+ * NVATTN_ERR_UNSUPPORTED for batches whose bounds allow 2^30 key tiles (128
+ * keys of a kv head) or more.  Results repeat bit for bit for a batch; another
+ * batch composition splits a context elsewhere and may move the last bits.
  * The launch uses the handle's workspace: calls on one handle are issued on
  * one stream, as for nvattn_paged_decode. */
 NVATTN_API nvattn_status nvattn_paged_decode_q8(

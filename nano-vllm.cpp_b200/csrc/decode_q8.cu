@@ -128,7 +128,7 @@ __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint
 
 // Where a walk over the CTA's run of tiles stands.
 struct Walk {
-  long long at;  // global tile index
+  int at;  // place in the line of tiles
   int seq, head, tile, ctx, n_tiles;
   int block, offset;  // where this warp's step of the tile lies in the sequence
 };
@@ -138,7 +138,7 @@ __device__ __forceinline__ int clamped_ctx(const Q8Params& p, int seq) {
 }
 __device__ __forceinline__ int tiles_of(int ctx) { return max(1, (ctx + kTile - 1) / kTile); }
 
-__device__ __forceinline__ void walk_next(const Q8Params& p, long long end, Walk& w) {
+__device__ __forceinline__ void walk_next(const Q8Params& p, int end, Walk& w) {
   ++w.at;
   w.offset += kTile;
   while (w.offset >= p.block_size) {
@@ -319,8 +319,8 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
   w.seq = run.seq;
   w.ctx = clamped_ctx(p, w.seq);
   w.n_tiles = tiles_of(w.ctx);
-  w.head = (int)((run.begin - run.seq_first) / (w.n_tiles + kUnitCost));
-  w.tile = (int)((run.begin - run.seq_first) % (w.n_tiles + kUnitCost)) - kUnitCost;
+  w.head = (run.begin - run.seq_first) / (w.n_tiles + kUnitCost);
+  w.tile = (run.begin - run.seq_first) % (w.n_tiles + kUnitCost) - kUnitCost;
   if (w.tile < 0) {  // the run begins before a unit's first tile
     w.at -= w.tile;
     w.tile = 0;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
   while (w.at < run.end) {
     // ---- one unit's part of the run ----
     const int seq = w.seq, head = w.head, first = w.tile, n_tiles = w.n_tiles, ctx = w.ctx;
-    const long long unit0 = w.at - w.tile;
+    const int unit0 = w.at - w.tile;
     const float up_g = load_q<kBf16>(p, seq, head, g, c, qa);
     // the lane's query rows from here on: 2c and 2c + 1
     const float up[2] = {__shfl_sync(0xffffffffu, up_g, 8 * c),
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
       __syncthreads();  // the merge buffer is free
     }
     if (!whole) {
-      const int c0 = (int)(unit0 / run.per), c1 = (int)((unit0 + n_tiles - 1) / run.per);
+      const int c0 = unit0 / run.per, c1 = (unit0 + n_tiles - 1) / run.per;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -631,6 +631,8 @@ nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, co
   p.tickets = h->part_tickets;
   p.status = h->status_dev;
   const long long tiles = (long long)n_seqs * p.Hkv * ((max_context_len + kTile - 1) / kTile);
+  if (tiles + (long long)n_seqs * p.Hkv * (1 + kUnitCost) >= tilesplit::kMaxPlaces)
+    return NVATTN_ERR_UNSUPPORTED;
   const int per_sm = tiles >= (long long)kFullGridTiles * kQ8CtasPerSm * h->sm_count
                          ? kQ8CtasPerSm : kQ8CtasPerSm - 1;
   const size_t smem = per_sm == kQ8CtasPerSm ? sizeof(Q8Smem) + 1024 : kTwoCtaSmem;

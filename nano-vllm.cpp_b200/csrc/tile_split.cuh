@@ -20,11 +20,16 @@
 namespace nvattn {
 namespace tilesplit {
 
+// (Places are 32-bit: the launchers refuse a batch whose host bounds allow
+// kMaxPlaces or more, and 64-bit divisions cost a short launch half a
+// microsecond.)
+constexpr long long kMaxPlaces = 1ll << 30;
+
 struct Run {
-  long long begin, end;  // places of this CTA's run
-  long long per;         // places per CTA
-  int seq;               // sequence that holds `begin`
-  long long seq_first;   // that sequence's first place
+  int begin, end;  // places of this CTA's run
+  int per;         // places per CTA
+  int seq;         // sequence that holds `begin`
+  int seq_first;   // that sequence's first place
 };
 
 // Shape of one sequence: `units` units of `tiles` places each.
@@ -38,38 +43,35 @@ template <class Shape>
 __device__ __forceinline__ Run find_run(int n_seqs, int cta, int n_ctas, int min_run,
                                         Shape shape) {
   const int lane = threadIdx.x & 31;
-  long long sum = 0, kept = 0;  // kept: the lane's last sequence's places
+  int sum = 0, kept = 0;  // kept: the lane's last sequence's places
   for (int s = lane; s < n_seqs; s += 32) {
     const SeqTiles t = shape(s);
-    kept = (long long)t.units * t.tiles;
+    kept = t.units * t.tiles;
     sum += kept;
   }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = __reduce_add_sync(0xffffffffu, sum);
   Run r;
-  r.per = max((sum + n_ctas - 1) / n_ctas, (long long)min_run);
-  r.begin = (long long)cta * r.per;
-  r.end = min(sum, r.begin + r.per);
+  r.per = max((int)(((unsigned)sum + n_ctas - 1) / (unsigned)n_ctas), min_run);
   r.seq = 0;
   r.seq_first = 0;
-  if (r.begin >= sum) {
-    r.end = r.begin;
-    return r;
-  }
-  long long before = 0;
+  const long long begin = (long long)cta * r.per;
+  r.begin = (int)min(begin, (long long)sum);
+  r.end = (int)min(begin + r.per, (long long)sum);
+  if (r.begin >= sum) return r;
+  int before = 0;
   for (int base = 0; base < n_seqs; base += 32) {
-    long long mine = kept;  // (one sequence per lane: nothing to read again)
+    int mine = kept;  // (one sequence per lane: nothing to read again)
     if (n_seqs > 32) {
       mine = 0;
       if (base + lane < n_seqs) {
         const SeqTiles t = shape(base + lane);
-        mine = (long long)t.units * t.tiles;
+        mine = t.units * t.tiles;
       }
     }
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
     const uint32_t past = __ballot_sync(0xffffffffu, before + incl > r.begin);

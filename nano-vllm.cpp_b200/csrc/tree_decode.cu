@@ -128,7 +128,7 @@ __device__ __forceinline__ int key_tiles(int ctx) {
 struct Segment {
   int seq, head, row_tile, j0, j1, n_tiles;
   SeqInfo info;
-  long long unit0;  // place of the unit's first tile
+  int unit0;  // place of the unit's first tile
 };
 
 constexpr int kMaxSlots = 13;
@@ -143,14 +143,14 @@ struct __align__(1024) TreeSmem {
   int skip;
   int last[2];
   Segment shared[2];  // units shared with other CTAs: at most the run's ends
-  long long per;      // places per CTA
+  int per;            // places per CTA
 };
 static_assert(sizeof(TreeSmem) + 1024 <= 227 * 1024, "shared memory");
 
 // Walks the segments of a run; every role walks the same ones.
 struct Walker {
   static constexpr int kUnitCost = kUnitCostKeys / kTile;
-  long long at, end;
+  int at, end;
   int entry, head;  // the unit that `at` lies in
   int offset;       // place of `at` in its unit
   SeqInfo info;
@@ -162,15 +162,15 @@ struct Walker {
     if (at >= end) return;
     info = entry_info(p, entry);
     const int span = key_tiles(info.ctx) + kUnitCost;
-    head = (int)((at - r.seq_first) / span);
-    offset = (int)((at - r.seq_first) % span);
+    head = (at - r.seq_first) / span;
+    offset = (at - r.seq_first) % span;
   }
 
   __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
     while (at < end) {
       const int tiles = key_tiles(info.ctx);
       const int left = tiles + kUnitCost - offset;
-      const int take = (int)min((long long)left, end - at);
+      const int take = min(left, end - at);
       const int j0 = max(offset - kUnitCost, 0), j1 = offset + take - kUnitCost;
       const bool some = j1 > j0;
       if (some)
@@ -718,8 +718,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __threadfence();
       named_barrier_sync(3, 2 * kGroup);
       auto ctas = [&](const Segment& u, int& c0, int& c1) {
-        c0 = (int)(u.unit0 / sm.per);
-        c1 = (int)((u.unit0 + u.n_tiles - 1) / sm.per);
+        c0 = u.unit0 / sm.per;
+        c1 = (u.unit0 + u.n_tiles - 1) / sm.per;
       };
       int c0, c1;
       if (tid < n_shared && grp == 0) {
@@ -804,6 +804,9 @@ nvattn_status launch_paged_tree_decode(nvattn_handle* h, int layer, int n_seqs, 
   p.mask_words = mask_words;
   p.max_context = max_context_len;
   p.row_tiles = (max_nodes * p.G + kRows - 1) / kRows;
+  if ((long long)n_seqs * p.row_tiles * p.Hkv *
+          ((long long)max_context_len / kTile + 1 + Walker::kUnitCost) >= tilesplit::kMaxPlaces)
+    return NVATTN_ERR_UNSUPPORTED;
   p.n_slots = h->n_slots;
   p.num_blocks = h->cfg.num_blocks;
   p.scale_log2 = h->cfg.scale * kLog2e;
