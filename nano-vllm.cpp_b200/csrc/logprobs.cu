@@ -21,9 +21,9 @@
 // logits), that limit is the k-th largest of kThreads interleaved subsets'
 // maxima; what is still too many (ties) is taken one after another.
 //
-// Measured: 256 rows of 151,936 f32 logits, top 5, 35.5 us (4.4 TB/s of logits,
+// Measured: 256 rows of 151,936 f32 logits, top 5, 34.9 us (4.5 TB/s of logits,
 // 69 % of the measured copy rate; the finish of the last rows is what the
-// loads do not cover); one bf16 row, top 20, 14.4 us (the chain of a tile or
+// loads do not cover); one bf16 row, top 20, 10.6 us (the chain of a tile or
 // two per warp, the cluster's hand-over and the finish).
 //
 // A row is one cluster of 1 to 8 CTAs, more where there are fewer rows
@@ -71,8 +71,8 @@ struct Smem {
   Sums part[kMaxCluster];        // CTA 0: the CTAs' sums
   Sums warp[kWarps];
   int tile[kMaxTop];             // the chosen tiles
-  uint32_t key[kMaxCandidates];
   int id[kMaxCandidates];
+  alignas(16) uint64_t order[kMaxCandidates];
   uint64_t best[kWarps];
   uint32_t floor_key;
   int count;
@@ -267,15 +267,23 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
   cluster_sync();
   if (cta != 0) return;
 
+  // ---- the k tiles that hold the top k; beside it, one thread (of the last
+  // warp, which ranks no tile unless there are many) the row's values ----
+  const int k_tiles = min(a.top_k, n_tiles);
   if (threadIdx.x == 0) {
+    sm.count = 0;
+    sm.floor_key = 0;
+  }
+  for (int i = n_tiles + threadIdx.x; i < (n_tiles + 3) / 4 * 4; i += kThreads)
+    sm.tile_key[i] = 0;  // precedes nothing
+  __syncthreads();
+  if (threadIdx.x == kThreads - 1) {
     Sums w = sm.part[0];
     for (int i = 1; i < n_ctas; ++i) w = join(w, sm.part[i]);
     const float m = w.m == -INFINITY ? 0.0f : w.m;
     const float log_s = logf(w.s);
     sm.m = m;
     sm.log_s = log_s;
-    sm.count = 0;
-    sm.floor_key = 0;
     if (a.entropy != nullptr) a.entropy[row_i] = log_s - w.t / w.s;
     if (a.tokens != nullptr) {
       if (!has_token) record_error(a.status, NVATTN_ERR_OUT_OF_RANGE, 95, row_i);
@@ -284,13 +292,6 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
     }
   }
   if (a.top_k <= 0) return;
-  __syncthreads();
-
-  // ---- the k tiles that hold the top k ----
-  const int k_tiles = min(a.top_k, n_tiles);
-  for (int i = n_tiles + threadIdx.x; i < (n_tiles + 3) / 4 * 4; i += kThreads)
-    sm.tile_key[i] = 0;  // precedes nothing
-  __syncthreads();
   for (int i = threadIdx.x; i < n_tiles; i += kThreads) {
     const uint32_t mine = sm.tile_key[i];
     const int rank = rank_of(sm.tile_key, n_tiles, mine, i);
@@ -344,10 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
         const int id = id_of<kBf16, kVec>(tile, lane, __ffs(reach) - 1);
         if (id < a.n_vocab) {
           const int at = atomicAdd(&sm.count, 1);
-          if (at < kMaxCandidates) {
-            sm.key[at] = ordered(load1<kBf16>(a, row, id));
-            sm.id[at] = id;
-          }
+          if (at < kMaxCandidates) sm.id[at] = id;
         }
       }
     }
@@ -357,23 +355,28 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
   }
   const long long out = (long long)row_i * a.top_k;
   if (n <= kMaxCandidates) {
+    // (key, ~id) as one 64-bit number is the order, largest first
+    for (int i = threadIdx.x; i < (n + 1) / 2 * 2; i += kThreads)
+      sm.order[i] = i < n ? (uint64_t)ordered(load1<kBf16>(a, row, sm.id[i])) << 32 |
+                                (uint32_t)~sm.id[i]
+                          : 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint32_t mine = sm.key[i];
-      const int id = sm.id[i];
+      const uint64_t mine = sm.order[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t other = sm.key[j];
-        rank += other > mine || (other == mine && sm.id[j] < id);
+#pragma unroll 4
+      for (int j = 0; j < n; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sm.order[j]);
+        rank += (o.x > mine) + (o.y > mine);
       }
       if (rank < a.top_k) {
-        a.top_ids[out + rank] = id;
-        a.top_logprobs[out + rank] = value_of(mine) - sm.m - sm.log_s;
+        a.top_ids[out + rank] = (int)~(uint32_t)mine;
+        a.top_logprobs[out + rank] = value_of((uint32_t)(mine >> 32)) - sm.m - sm.log_s;
       }
     }
     return;
   }
   // Too many to rank at once: the first, then the first after it, and so on.
-  // (key, ~id) as one 64-bit number is the order, largest first.
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top_k; ++k) {
     uint64_t best = 0;
