@@ -475,8 +475,9 @@ NVATTN_API nvattn_status nvattn_paged_prefill_rows(
  * NVATTN_ERR_UNSUPPORTED for batches whose bounds allow 2^30 key tiles (64
  * keys each, counted per kv head and 128 query rows) or more.
  * Results repeat bit for bit for a batch; another batch composition splits a
- * context elsewhere and may move the last bits.  The launch uses the handle's workspace: calls on one handle are issued on
- * one stream, as for nvattn_paged_decode. */
+ * context elsewhere and may move the last bits.  The launch uses the handle's
+ * workspace: calls on one handle are issued on one stream, as for
+ * nvattn_paged_decode. */
 NVATTN_API nvattn_status nvattn_paged_tree_decode(
     nvattn_handle* h, int layer, int n_seqs, int n_nodes, const void* q_dev, nvattn_dtype dtype,
     const int32_t* cu_nodes_dev, const uint64_t* tree_mask_dev, int mask_words, int max_nodes,

@@ -218,7 +218,9 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
     }
     r.s += (s[0] + s[1]) + (s[2] + s[3]);
     r.t += (t[0] + t[1]) + (t[2] + t[3]);
-    if (has_token) {
+    // (a tile whose maximum lies below the token's logit has nothing before it:
+    // most tiles, where the token is a likely one)
+    if (has_token && value_of(key) >= xt) {
       int n = 0;
       if (token >= (tile + 1) * kTile) {  // equals come before the token
 #pragma unroll
