@@ -54,7 +54,7 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kRows = 128;
-constexpr int kTile = 64;  // keys per tile
+constexpr int kTile = 64;  // keys per tile (a mask word's)
 constexpr int kGroup = 128;  // softmax threads of one group
 constexpr int kThreads = 3 * kGroup;
 // Registers per thread: 168 at launch (384 threads); the softmax groups take
@@ -137,7 +137,8 @@ struct __align__(1024) TreeSmem {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2], s_full[4], p_full[4], o_done;
   float m[2][kRows], l[2][kRows];  // the groups' references and sums at a unit's end
-  uint32_t bad[2][4];  // [group]: keys of its tile whose V row holds a NaN or an infinity
+  // [group][tile with nodes, mod 3]: keys whose V row holds a NaN or an infinity
+  uint32_t bad[2][3][kTile / 32];
   uint32_t tmem_base;
   int abort_flag;
   int skip;
@@ -215,8 +216,20 @@ __device__ __forceinline__ void write_dims(const TreeParams& p, long long at, co
   }
 }
 
-// Merges the partials of a unit that CTAs c0..c1 share, in CTA order: a lane
-// per row, the eight softmax warps split the dims (and the rows, 32 each).
+// A softmax warp's share of `rows` rows of 128 dims: a lane per row, `dims` dims
+// from d0.  Where the rows are few the eight warps split the dims.
+struct Share {
+  int row, d0, dims;
+};
+__device__ __forceinline__ Share share_of(int rows) {
+  const int w = ((int)threadIdx.x >> 5) - 4;  // 0..7
+  const int quads = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int dims = kD * quads / 8;
+  return {(w % quads) * 32 + ((int)threadIdx.x & 31), (w / quads) * dims, dims};
+}
+
+// Merges the partials of a unit that CTAs c0..c1 share, in CTA order: split
+// over the softmax warps (share_of).
 // Four partials at a time, with all of their loads in flight together: the
 // reads are bound by their latency where the rows are few, and by what one SM
 // reads from L2 (about 110 GB/s) where they are many.
@@ -224,17 +237,15 @@ template <bool kF32>
 __device__ __forceinline__ void merge_parts(const TreeParams& p, const Segment& seg, int c0,
                                             int c1) {
   constexpr int kAtOnce = 4, kDims = 16;
-  const int lane = threadIdx.x & 31, w = ((int)threadIdx.x >> 5) - 4;  // 0..7
   const int rows = min(seg.info.n * p.G - seg.row_tile * kRows, kRows);
-  const int quads = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-  const int r = (w % quads) * 32 + lane;
-  const int dims = kD * quads / 8, d0 = (w / quads) * dims;
+  const Share share = share_of(rows);
+  const int r = share.row;
   if (r >= rows) return;
   const int row = seg.row_tile * kRows + r;
   const long long io = ((long long)(seg.info.node0 + row / p.G) * p.Hq +
                         (long long)seg.head * p.G + row % p.G) * kD;
 #pragma unroll 1
-  for (int d = d0; d < d0 + dims; d += kDims) {
+  for (int d = share.d0; d < share.d0 + share.dims; d += kDims) {
     float o[kDims], M = -INFINITY, L = 0.0f;
 #pragma unroll
     for (int i = 0; i < kDims; ++i) o[i] = 0.0f;
@@ -312,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], kF32 ? 8 : 1);
       mbar_init(&sm.q_empty[i], 1);
-      for (int k = 0; k < 4; ++k) sm.bad[i][k] = 0;
+      for (int k = 0; k < 3; ++k) sm.bad[i][k][0] = sm.bad[i][k][1] = 0;
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(&sm.s_full[i], 1);
@@ -482,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t c2 = pack2(p.scale_log2, p.scale_log2);
     int g = 0;  // tiles of the run before the segment
     int n_shared = 0;
+    int n_special = 0;  // tiles with nodes (of this group) so far
     for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
       const int n_rows = seg.info.n * p.G;
       const int row = seg.row_tile * kRows + r;
@@ -492,27 +504,44 @@ __global__ void __launch_bounds__(kThreads, 1)
           ((long long)node * p.Hq + (long long)seg.head * p.G + (real ? row % p.G : 0)) * kD;
       const int first = seg.info.ctx - seg.info.n;  // position of the sequence's first node
       if constexpr (kF32) {
-        // ---- query operand: this thread's row, dims [64 grp, 64 grp + 64)
-        // (the MMAs that read the last one are complete: o_done) ----
-        if (warp_real) {
-          uint8_t* q_row = sm.operands + grp * (kQTermBytes / 2) + r * 128;
-          const float4* src =
-              reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + io + 64 * grp);
-          float4 v[16];
+        // ---- query operand (the MMAs that read the last one are complete:
+        // o_done), 16 dims at a time ----
+        const int q_rows = min(n_rows - seg.row_tile * kRows, kRows);
+        const Share share = share_of(q_rows);
+        if ((share.row & ~31) < q_rows) {
+          const bool q_real = share.row < q_rows;
+          const int q_row = seg.row_tile * kRows + (q_real ? share.row : 0);
+          const float4* src = reinterpret_cast<const float4*>(
+              static_cast<const float*>(p.q) +
+              ((long long)(seg.info.node0 + q_row / p.G) * p.Hq + (long long)seg.head * p.G +
+               q_row % p.G) * kD + share.d0);
+          uint8_t* dst = sm.operands + share.row * 128;
+          float4 next[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            v[i] = real ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int i = 0; i < 4; ++i) next[i] = src[i];
+#pragma unroll 1
+          for (int d = 0; d < share.dims; d += 16) {
+            float4 v[4];
 #pragma unroll
-          for (int t = 0; t < kQ; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint4 w;
-              split_term(v[2 * i].x, v[2 * i].y, w.x);
-              split_term(v[2 * i].z, v[2 * i].w, w.y);
-              split_term(v[2 * i + 1].x, v[2 * i + 1].y, w.z);
-              split_term(v[2 * i + 1].z, v[2 * i + 1].w, w.w);
-              *reinterpret_cast<uint4*>(q_row + t * kQTermBytes + ((i ^ (r & 7)) << 4)) = w;
+            for (int i = 0; i < 4; ++i) {
+              v[i] = q_real ? next[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (d + 16 < share.dims) next[i] = src[(d + 16) / 4 + i];
             }
+            uint8_t* half = dst + ((share.d0 + d) >> 6) * (kQTermBytes / 2);
+            const int chunk = ((share.d0 + d) & 63) >> 3;  // of 8 dims
+#pragma unroll
+            for (int t = 0; t < kQ; ++t)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint4 w;
+                split_term(v[2 * i].x, v[2 * i].y, w.x);
+                split_term(v[2 * i].z, v[2 * i].w, w.y);
+                split_term(v[2 * i + 1].x, v[2 * i + 1].y, w.z);
+                split_term(v[2 * i + 1].z, v[2 * i + 1].w, w.w);
+                *reinterpret_cast<uint4*>(half + t * kQTermBytes +
+                                          (((chunk + i) ^ (share.row & 7)) << 4)) = w;
+              }
+          }
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -526,40 +555,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int gj = g + j;
         const int col0 = (seg.j0 + j) * kT;
         const uint32_t s_col = lanes + kColS + (gj % kBufs) * kColsS;
-        mbar_wait(&sm.s_full[gj % kBufs], (gj / kBufs) & 1, p.status, abort_flag, 110);
-        tc_fence_after();
         const bool special = col0 + kT > first;  // the tile holds nodes (or keys past the end)
-        uint64_t allowed[kT / 64];               // which of its keys the row attends
-        if (special) {
-#pragma unroll
-          for (int h = 0; h < kT / 64; ++h) {
-            const int rel = col0 + 64 * h - first;  // the first key's place among the nodes
-            uint64_t w = 0;
-            if (rel <= -64) {
-              w = ~0ull;
-            } else if (real) {
-              const uint64_t* words = p.mask + (long long)node * p.mask_words;
-              if (rel < 0) {
-                w = (words[0] << -rel) | ((1ull << -rel) - 1);
-              } else {
-                const int q = rel >> 6, sh = rel & 63;
-                if (q < p.mask_words) w = words[q] >> sh;
-                if (sh > 0 && q + 1 < p.mask_words) w |= words[q + 1] << (64 - sh);
-              }
+        uint64_t allowed = 0;                    // which of its keys the row attends
+        if (special) {  // (before the wait for its scores, which it hides behind)
+          const int rel = col0 - first;  // the first key's place among the nodes
+          if (rel <= -kT) {
+            allowed = ~0ull;
+          } else if (real) {
+            const uint64_t* words = p.mask + (long long)node * p.mask_words;
+            if (rel < 0) {
+              allowed = (words[0] << -rel) | ((1ull << -rel) - 1);
+            } else {
+              const int q = rel >> 6, sh = rel & 63;
+              if (q < p.mask_words) allowed = words[q] >> sh;
+              if (sh > 0 && q + 1 < p.mask_words) allowed |= words[q + 1] << (64 - sh);
             }
-            const int here = seg.info.ctx - col0 - 64 * h;  // keys of the context from here on
-            if (here < 64) w = here > 0 ? w & ((1ull << here) - 1) : 0;
-            allowed[h] = w;
           }
+          const int here = seg.info.ctx - col0;  // keys of the context from here on
+          if (here < kT) allowed &= (1ull << here) - 1;
           // V rows of nodes that hold a NaN or an infinity: 0 * NaN would
           // reach the rows whose masks leave the node out.  Such a row is
           // zeroed and noted, and makes the rows that attend it NaN.  Slots
           // past the context may hold anything and are zeroed.
           const int slot = v_slot(gj);
           mbar_wait(&sm.full[slot], v_parity(gj), p.status, abort_flag, 111);
-#pragma unroll
-          for (int i = 0; i < kT / 64; ++i) {
-            const int t = (tid >> 1) + 64 * i;  // key of the tile; two threads, a dim half each
+          volatile uint32_t* bad_now = sm.bad[grp][n_special % 3];
+          {
+            const int t = tid >> 1;  // key of the tile; two threads, a dim half each
             uint4* v = reinterpret_cast<uint4*>(ring + slot * kTileBytes + (tid & 1) * kHalfBytes +
                                                 t * 128);
             const bool past = col0 + t >= seg.info.ctx;
@@ -574,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const uint32_t votes = __ballot_sync(0xffffffffu, bad && !past && col0 + t >= first);
             bad = (votes >> (lane & ~1)) & 3u;
-            if (bad && (tid & 1) == 0) atomicOr(&sm.bad[grp][t >> 5], 1u << (t & 31));
+            if (bad && (tid & 1) == 0)
+              atomicOr(&sm.bad[grp][n_special % 3][t >> 5], 1u << (t & 31));
             if (bad || past) {
 #pragma unroll
               for (int k = 0; k < 8; ++k) v[k] = make_uint4(0, 0, 0, 0);
@@ -582,15 +605,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async_smem();
           named_barrier_sync(1 + grp, kGroup);
-#pragma unroll
-          for (int h = 0; h < kT / 64; ++h) {
-            const uint64_t bad_keys = (uint64_t)sm.bad[grp][2 * h + 1] << 32 | sm.bad[grp][2 * h];
-            if (bad_keys & allowed[h]) l = __uint_as_float(0x7fc00000u);
-          }
-          named_barrier_sync(1 + grp, kGroup);
-          // (set again in the group's next tile, whose S follows this P)
-          if (tid < 4) sm.bad[grp][tid] = 0;
+          const uint64_t bad_keys = (uint64_t)bad_now[1] << 32 | bad_now[0];
+          if (bad_keys & allowed) l = __uint_as_float(0x7fc00000u);
+          // Cleared for the tile with nodes after the next one: every thread has
+          // read it (before this barrier), and none sets it before the next one.
+          if (tid < 2) sm.bad[grp][(n_special + 2) % 3][tid] = 0;
+          ++n_special;
         }
+        mbar_wait(&sm.s_full[gj % kBufs], (gj / kBufs) & 1, p.status, abort_flag, 110);
+        tc_fence_after();
         if (warp_real) {
           float x[kT];
 #pragma unroll
@@ -600,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (special) {
 #pragma unroll
             for (int i = 0; i < kT; ++i)
-              x[i] = (allowed[i >> 6] >> (i & 63)) & 1 ? x[i] : -INFINITY;
+              x[i] = (allowed >> i) & 1 ? x[i] : -INFINITY;
           }
           float tops[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll

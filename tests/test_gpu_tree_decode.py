@@ -176,6 +176,27 @@ def test_padded_nodes_and_nan_rows(cuda, bf16):
     Q.check(np.where(bad, want, got), want, tol, bf16)
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+def test_nan_rows_in_every_other_tile(cuda, bf16):
+    """Tiles with nodes one after another (five per unit, several units per
+    CTA); in every other 64 positions the nodes' V rows are NaN and no mask
+    names them: what is noted of one tile is not taken for another's."""
+    Hq, Hkv, n_seqs, N = 1, 1, 200, 250
+    c = tree_case(21, Hq, Hkv, [N + 3] * n_seqs, [N] * n_seqs, bs=128, words=4)
+    at = np.arange(3, N + 3)
+    for s in range(n_seqs):
+        pad = (at // 64 + s) % 2 == 0
+        c["masks"][s][:, :N][:, pad] = False
+        c["v"][0, Q.slots_of(c["bt"][s], N + 3, 128)[3:][pad]] = 0x7fc0
+    clean = dict(c, v=c["v"].copy())
+    clean["v"][~np.isfinite(O.bf16_to_f32(clean["v"]))] = 0
+    h, got, q = run(c, bf16)
+    h.check_device()
+    Q.check(got, *expect(clean, q, bf16), bf16)
+    for _ in range(5):
+        assert np.array_equal(run(c, bf16, h)[1], got)
+
+
 def test_one_node_is_the_decode(cuda):
     """A tree of one node is a decode step."""
     torch = torch_()
