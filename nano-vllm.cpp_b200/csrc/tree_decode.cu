@@ -216,6 +216,53 @@ __device__ __forceinline__ void write_dims(const TreeParams& p, long long at, co
   }
 }
 
+// 32 dims from `d` of 32 rows of a unit's sequence, rows row0 + lane (those
+// below n_rows).  Lanes trade 16-byte chunks in fours, so that four of them
+// write 64 consecutive bytes of one row: a lane alone would write 16 bytes to
+// a line of its own.
+template <bool kF32>
+__device__ __forceinline__ void write_rows(const TreeParams& p, const Segment& seg, int row0,
+                                           int n_rows, int d, const float (&o)[32]) {
+  constexpr int kPer = kF32 ? 4 : 8;  // elements per chunk
+  const int lane = threadIdx.x & 31, log_g = 31 - __clz(p.G);
+#pragma unroll
+  for (int set = 0; set < 32; set += 4 * kPer) {
+    uint32_t u[4][4];  // [chunk], then [row of the four]
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = set + kPer * i + e * (kPer / 4);
+        u[i][e] = kF32 ? __float_as_uint(o[x]) : pack_bf16x2(o[x], o[x + kPer / 4 - 1]);
+      }
+#pragma unroll
+    for (int stage = 1; stage <= 2; ++stage) {
+      const bool odd = lane & stage;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i & stage) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t &a = u[i][e], &b = u[i | stage][e];
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? a : b, stage);
+          if (odd) a = other; else b = other;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + (lane & ~3) + i;
+      if (row < n_rows) {
+        const long long at = ((long long)(seg.info.node0 + (row >> log_g)) * p.Hq +
+                              (long long)seg.head * p.G + (row & (p.G - 1))) * kD +
+                             d + set + kPer * (lane & 3);
+        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + at * (kF32 ? 4 : 2)) =
+            make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
+      }
+    }
+  }
+}
+
 // A softmax warp's share of `rows` rows of 128 dims: a lane per row, `dims` dims
 // from d0.  Where the rows are few the eight warps split the dims.
 struct Share {
@@ -254,9 +301,10 @@ __device__ __forceinline__ void merge_parts(const TreeParams& p, const Segment& 
       float v[kAtOnce][kDims], m[kAtOnce], l[kAtOnce];
 #pragma unroll
       for (int e = 0; e < kAtOnce; ++e) {
-        // (the first CTA left its part in its second place: tile_split.cuh;
-        // behind the last part: that part again, with no weight)
-        const int i = min(k + e, c1);
+        m[e] = -INFINITY;
+        if (k + e > c1) continue;
+        // (the first CTA left its part in its second place: tile_split.cuh)
+        const int i = k + e;
         const float* src = p.part + ((long long)i * 2 + (i == c0)) * kTreePartFloats + r;
         m[e] = __ldcg(src + kD * kRows);
         l[e] = __ldcg(src + kD * kRows + kRows);
@@ -316,6 +364,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto v_parity = [](int g) { return (uint32_t)(g / kSlotsV) & 1u; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    if constexpr (!kF32) tma_prefetch_desc(&tm_q);
     for (int i = 0; i < kSlotsK + kSlotsV; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 1);
@@ -362,8 +413,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_dec<kControlRegs>();
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
       // (evict_first also where a kv head has several row tiles, whose reads
       // come close together: 16 ragged drafts took 109 us with it, 117 without)
       const uint64_t policy = l2_policy_evict_first();
@@ -494,14 +543,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = 0;  // tiles of the run before the segment
     int n_shared = 0;
     int n_special = 0;  // tiles with nodes (of this group) so far
-    for (int n_seg = 0; walk.next(p, seg); ++n_seg) {
+    bool more = walk.next(p, seg);
+    for (int n_seg = 0; more; ++n_seg) {
       const int n_rows = seg.info.n * p.G;
       const int row = seg.row_tile * kRows + r;
       const bool real = row < n_rows;
       const bool warp_real = seg.row_tile * kRows + quad * 32 < n_rows;
       const int node = seg.info.node0 + (real ? row / p.G : 0);
-      const long long io =
-          ((long long)node * p.Hq + (long long)seg.head * p.G + (real ? row % p.G : 0)) * kD;
       const int first = seg.info.ctx - seg.info.n;  // position of the sequence's first node
       if constexpr (kF32) {
         // ---- query operand (the MMAs that read the last one are complete:
@@ -690,6 +738,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- the unit's end: each group combines O_0 and O_1 for half of the dims ----
       sm.m[grp][r] = m;
       sm.l[grp][r] = l;
+      Segment next_seg;
+      more = walk.next(p, next_seg);  // (while the last P V runs)
       mbar_wait(&sm.o_done, n_seg & 1, p.status, abort_flag, 113);
       tc_fence_after();
       named_barrier_sync(3, 2 * kGroup);
@@ -713,10 +763,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            o[i] = (has0 ? __uint_as_float(w0[i]) * f0 : 0.0f) +
-                   (has1 ? __uint_as_float(w1[i]) * f1 : 0.0f);
+            o[i] = ((has0 ? __uint_as_float(w0[i]) * f0 : 0.0f) +
+                    (has1 ? __uint_as_float(w1[i]) * f1 : 0.0f)) * inv;
           if (whole) {
-            if (real) write_dims<kF32, 32>(p, io + c, o, inv);
+            write_rows<kF32>(p, seg, seg.row_tile * kRows + quad * 32, n_rows, c, o);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) part[(c + i) * kRows + r] = o[i];
@@ -735,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (threadIdx.x == kGroup) sm.shared[n_shared] = seg;
         ++n_shared;
       }
+      seg = next_seg;
     }
     // ---- publish the partials; merge the units whose last one this is ----
     if (n_shared > 0) {
