@@ -52,8 +52,7 @@ constexpr int kStep = 32;                // tokens per warp step
 constexpr int kTile = kWarps * kStep;    // tokens per CTA tile
 constexpr int kStages = 2;
 constexpr int kRows = 8;                 // query rows per unit (GQA group, padded)
-constexpr int kMergeRows = 2;            // rows the warps merge at a time
-static_assert(kWarps == 2 * kMergeRows, "a merge takes two warps per row");
+static_assert(kRows == 2 * kWarps && kWarps == 4, "merges: two rows per warp, or two warps per row");
 // A unit's start and end (its queries, the warps' merge, its rows or partial)
 // cost about as much as this many tiles, and the split counts them as such.
 constexpr int kUnitCost = 2;
@@ -64,7 +63,7 @@ constexpr int kUnitCost = 2;
 constexpr int kFullGridTiles = 48;
 // Shared memory of a launch with two CTAs per SM: more than a third of an SM's,
 // so that no SM takes three while another takes one.
-constexpr int kTwoCtaSmem = 96 * 1024;
+constexpr size_t kTwoCtaSmem = 96 * 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;           // log2: rescale only past 2^8
 static_assert(128 % kStep == 0, "a step must not cross a block (block sizes are multiples of 128)");
@@ -94,12 +93,19 @@ struct __align__(1024) Q8Smem {
   float ks[kWarps][kStages][kStep];
   float vs[kWarps][kStages][kStep];
   float4 tok[kWarps][kStep];  // {score factor, log2 s_v, 1 / s_v, 0} of the step's tokens
-  float o[kWarps][kMergeRows][kD];  // of the rows being merged
   float m[kWarps][kRows], l[kWarps][kRows];
+  const float4* o[kWarps];  // the warps' rows at a unit's end: [row][kD / 4], see merge_chunk
   uint64_t full[kWarps][kStages];
   int abort_flag;
   int last;
 };
+
+// Where the q-th four dims of row `row` lie in the row, while the warps merge:
+// as that, the eight lanes that write (or read) at a time hit distinct banks.
+__device__ __forceinline__ int merge_chunk(int row, int q) {
+  return q ^ ((row >> 1) | (q >> 4 << 2));
+}
+static_assert(kRows * kD * 4 == kStep * kD, "a warp's rows fill a stage of K");
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -245,14 +251,22 @@ __device__ __forceinline__ void fma4(float4& o, const float4& a, float f) {
 }
 
 // Merges the partials of a unit that CTAs c0..c1 share, in CTA order.  A warp
-// per row, 32 partials at a time: a lane per partial for the factors, then
-// four dimensions per lane, the partials' loads independent of one another.
-template <bool kBf16>
+// takes kR rows at a time, and 32 partials: a lane per partial for the factors,
+// then four dimensions per lane.  kEarly partials' rows are read together with
+// the factors: the launch ends with this, and each dependent read is about half
+// a microsecond.
+template <bool kBf16, int kR, int kEarly>
 __device__ __forceinline__ void merge_parts(const Q8Params& p, int seq, int head, int c0, int c1) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < p.G; r += kWarps) {
-    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float M = -INFINITY, L = 0.0f;
+  for (int r0 = warp; r0 < p.G; r0 += kWarps * kR) {
+    float4 O[kR];
+    float M[kR], L[kR];
+#pragma unroll
+    for (int x = 0; x < kR; ++x) {
+      O[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      M[x] = -INFINITY;
+      L[x] = 0.0f;
+    }
     for (int base = c0; base <= c1; base += 32) {
       const int n = min(c1 + 1 - base, 32);
       // (the first CTA left its part in its second place: tile_split.cuh)
@@ -261,34 +275,65 @@ __device__ __forceinline__ void merge_parts(const Q8Params& p, int seq, int head
       auto at = [&](int i) {
         return i == 0 ? q : q + step + (long long)(i - 1) * 2 * kQ8PartFloats;
       };
-      float m = -INFINITY, l = 0.0f;
-      if (lane < n) {
-        m = __ldcg(at(lane) + kRows * kD + r);
-        l = __ldcg(at(lane) + kRows * kD + kRows + r);
+      auto load = [&](int i, int r) {
+        return __ldcg(reinterpret_cast<const float4*>(at(i) + r * kD) + lane);
+      };
+      float m[kR], l[kR], f[kR];
+      float4 v[kR][kEarly > 0 ? kEarly : 1];
+#pragma unroll
+      for (int x = 0; x < kR; ++x) {
+        const int r = r0 + kWarps * x;
+        m[x] = -INFINITY;
+        l[x] = 0.0f;
+        if (r >= p.G) break;
+        if (lane < n) {
+          m[x] = __ldcg(at(lane) + kRows * kD + r);
+          l[x] = __ldcg(at(lane) + kRows * kD + kRows + r);
+        }
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i)
+          if (i < n) v[x][i] = load(i, r);
       }
-      float top = fmaxf(m, M);
 #pragma unroll
-      for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-      const float old = M == -INFINITY ? 1.0f : fast_exp2(M - top);
-      const float f = m == -INFINITY ? 1.0f : fast_exp2(m - top);
-      float s = l * f;
+      for (int x = 0; x < kR; ++x) {
+        float top = fmaxf(m[x], M[x]);
 #pragma unroll
-      for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      L = fmaf(L, old, s);
-      M = top;
-      O = make_float4(O.x * old, O.y * old, O.z * old, O.w * old);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i)
-        fma4(O, __ldcg(reinterpret_cast<const float4*>(at(i) + r * kD) + lane),
-             __shfl_sync(0xffffffffu, f, i));
+        for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+        const float old = M[x] == -INFINITY ? 1.0f : fast_exp2(M[x] - top);
+        f[x] = m[x] == -INFINITY ? 1.0f : fast_exp2(m[x] - top);
+        float s = l[x] * f[x];
+#pragma unroll
+        for (int y = 16; y >= 1; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
+        L[x] = fmaf(L[x], old, s);
+        M[x] = top;
+        O[x] = make_float4(O[x].x * old, O[x].y * old, O[x].z * old, O[x].w * old);
+      }
+#pragma unroll
+      for (int x = 0; x < kR; ++x) {
+        const int r = r0 + kWarps * x;
+        if (r >= p.G) break;
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i) {
+          const float fi = __shfl_sync(0xffffffffu, f[x], i);
+          if (i < n) fma4(O[x], v[x][i], fi);
+        }
+#pragma unroll(kR > 1 ? 4 : 8)
+        for (int i = kEarly; i < n; ++i)
+          fma4(O[x], load(i, r), __shfl_sync(0xffffffffu, f[x], i));
+      }
     }
-    const float o[4] = {O.x, O.y, O.z, O.w};
-    write_out<kBf16>(p, seq, head, r, 4 * lane, o, L);
+#pragma unroll
+    for (int x = 0; x < kR; ++x) {
+      const int r = r0 + kWarps * x;
+      if (r >= p.G) break;
+      const float o[4] = {O[x].x, O[x].y, O[x].z, O[x].w};
+      write_out<kBf16>(p, seq, head, r, 4 * lane, o, L[x]);
+    }
   }
 }
 
-template <bool kBf16>
-__global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
+template <bool kBf16, int kCtas>  // kCtas: CTAs per SM
+__global__ void __launch_bounds__(kThreads, kCtas)
     decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, Q8Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -518,12 +563,13 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
         }
         __syncwarp();  // every lane has read the stage
       }
-      if (ahead.at < run.end) issue();
       walk_next(p, run.end, w);
       ++done;
-    } while (w.at < run.end && w.tile != 0);
+      if (w.at >= run.end || w.tile == 0) break;  // the unit's last: issued after the merge
+      if (ahead.at < run.end) issue();
+    } while (true);
 
-    // ---- merge the warps: two warps per row, two dimensions per lane ----
+    // ---- merge the warps ----
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -536,42 +582,42 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
     }
     const bool whole = first == 0 && done == n_tiles;
     float* part = p.part + ((long long)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * kQ8PartFloats;
-    for (int r0 = 0; r0 < p.G; r0 += kMergeRows) {
-      if (2 * c == r0) {
+    // The warp's rows go to the K part of the stage that is filled next (free:
+    // the last tile's load has not been issued); a warp then merges two rows.
+    float4* rows = reinterpret_cast<float4*>(sm.ring[warp].k[issued % kStages]);
+    if (lane == 0) sm.o[warp] = rows;
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4*>(&sm.o[warp][r][16 * pr + 4 * j]) = make_float4(
-                o[2 * j][r], o[2 * j][2 + r], o[2 * j + 1][r], o[2 * j + 1][2 + r]);
+      for (int j = 0; j < 4; ++j)
+        rows[(2 * c + r) * (kD / 4) + merge_chunk(2 * c + r, 4 * pr + j)] =
+            make_float4(o[2 * j][r], o[2 * j][2 + r], o[2 * j + 1][r], o[2 * j + 1][2 + r]);
+    __syncthreads();
+    for (int r = warp; r < p.G; r += kWarps) {
+      float M = -INFINITY, L = 0.0f;
+      float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.m[i][r]);
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const float f = sm.m[i][r] == -INFINITY ? 1.0f : fast_exp2(sm.m[i][r] - M);
+        fma4(O, sm.o[i][r * (kD / 4) + merge_chunk(r, lane)], f);
+        L = fmaf(sm.l[i][r], f, L);
       }
-      __syncthreads();
-      const int r = r0 + (warp & 1), d = 64 * (warp >> 1) + 2 * lane;
-      if (r < p.G) {
-        float M = -INFINITY, L = 0.0f;
-        float O[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.m[i][r]);
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-          const float f = sm.m[i][r] == -INFINITY ? 1.0f : fast_exp2(sm.m[i][r] - M);
-          const float2 v = *reinterpret_cast<const float2*>(&sm.o[i][warp & 1][d]);
-          O[0] = fmaf(v.x, f, O[0]);
-          O[1] = fmaf(v.y, f, O[1]);
-          L = fmaf(sm.l[i][r], f, L);
-        }
-        if (whole) {
-          write_out<kBf16>(p, seq, head, r, d, O, L);
-        } else {
-          *reinterpret_cast<float2*>(part + r * kD + d) = make_float2(O[0], O[1]);
-          if (d == 0) {
-            part[kRows * kD + r] = M;
-            part[kRows * kD + kRows + r] = L;
-          }
+      if (whole) {
+        const float y[4] = {O.x, O.y, O.z, O.w};
+        write_out<kBf16>(p, seq, head, r, 4 * lane, y, L);
+      } else {
+        *reinterpret_cast<float4*>(part + r * kD + 4 * lane) = O;
+        if (lane == 0) {
+          part[kRows * kD + r] = M;
+          part[kRows * kD + kRows + r] = L;
         }
       }
-      __syncthreads();  // the merge buffer is free
     }
+    fence_proxy_async_smem();  // before the next copy into the stage
+    __syncthreads();           // the rows have been read
+    if (ahead.at < run.end) issue();
     if (!whole) {
       const int c0 = unit0 / run.per, c1 = (unit0 + n_tiles - 1) / run.per;
       __threadfence();
@@ -584,7 +630,10 @@ __global__ void __launch_bounds__(kThreads, kQ8CtasPerSm)
       __syncthreads();
       if (sm.last) {
         __threadfence();
-        merge_parts<kBf16>(p, seq, head, c0, c1);
+        if constexpr (kCtas == 2)
+          merge_parts<kBf16, 2, 4>(p, seq, head, c0, c1);
+        else  // (three CTAs per SM have no registers for that)
+          merge_parts<kBf16, 1, 0>(p, seq, head, c0, c1);
       }
       __syncthreads();  // sm.last is free
     }
@@ -635,26 +684,26 @@ nvattn_status launch_paged_decode_q8(nvattn_handle* h, int layer, int n_seqs, co
     return NVATTN_ERR_UNSUPPORTED;
   const int per_sm = tiles >= (long long)kFullGridTiles * kQ8CtasPerSm * h->sm_count
                          ? kQ8CtasPerSm : kQ8CtasPerSm - 1;
-  const size_t smem = per_sm == kQ8CtasPerSm ? sizeof(Q8Smem) + 1024 : kTwoCtaSmem;
-  static_assert(kQ8CtasPerSm == 3 && sizeof(Q8Smem) + 1024 <= kTwoCtaSmem, "two per SM");
-  static_assert(kQ8CtasPerSm * (sizeof(Q8Smem) + 2048) <= 228 * 1024, "CTAs per SM");
+  using Kernel = void (*)(const CUtensorMap, const CUtensorMap, Q8Params);
+  constexpr size_t smem_full = sizeof(Q8Smem) + 1024;
+  static_assert(kQ8CtasPerSm == 3 && 3 * (smem_full + 1024) <= 228 * 1024, "three per SM");
+  static_assert(smem_full <= kTwoCtaSmem && 2 * (kTwoCtaSmem + 1024) <= 228 * 1024, "two per SM");
+  const bool bf16 = dtype == NVATTN_DTYPE_BF16, full = per_sm == kQ8CtasPerSm;
+  const Kernel kernels[2][2] = {{decode_q8_kernel<false, 2>, decode_q8_kernel<false, 3>},
+                                {decode_q8_kernel<true, 2>, decode_q8_kernel<true, 3>}};
   // (atomic: handles on different threads may launch at the same time)
   static std::atomic<unsigned long long> attr_set_mask{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return NVATTN_ERR_CUDA;
   if (dev >= 64 || !(attr_set_mask.load(std::memory_order_relaxed) & (1ull << dev))) {
-    if (cudaFuncSetAttribute(decode_q8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kTwoCtaSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(decode_q8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kTwoCtaSmem) != cudaSuccess)
-      return NVATTN_ERR_CUDA;
+    for (int i = 0; i < 4; ++i)
+      if (cudaFuncSetAttribute(kernels[i >> 1][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)((i & 1) ? smem_full : kTwoCtaSmem)) != cudaSuccess)
+        return NVATTN_ERR_CUDA;
     if (dev < 64) attr_set_mask.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  const int grid = per_sm * h->sm_count;
-  if (dtype == NVATTN_DTYPE_BF16)
-    decode_q8_kernel<true><<<grid, kThreads, smem, stream>>>(tk, tv, p);
-  else
-    decode_q8_kernel<false><<<grid, kThreads, smem, stream>>>(tk, tv, p);
+  kernels[bf16][full]<<<per_sm * h->sm_count, kThreads, full ? smem_full : kTwoCtaSmem,
+                        stream>>>(tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? NVATTN_OK : NVATTN_ERR_CUDA;
 }
 
