@@ -52,7 +52,7 @@ constexpr int kStep = 32;                // tokens per warp step
 constexpr int kTile = kWarps * kStep;    // tokens per CTA tile
 constexpr int kStages = 2;
 constexpr int kRows = 8;                 // query rows per unit (GQA group, padded)
-static_assert(kRows == 2 * kWarps && kWarps == 4, "merges: two rows per warp, or two warps per row");
+static_assert(kRows == 2 * kWarps, "merge_parts: two rows per warp");
 // A unit's start and end (its queries, the warps' merge, its rows or partial)
 // cost about as much as this many tiles, and the split counts them as such.
 constexpr int kUnitCost = 2;

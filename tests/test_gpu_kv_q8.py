@@ -12,7 +12,6 @@ import q8_util as Q
 from gpu_util import dev, handle
 
 pytestmark = pytest.mark.gpu
-BF16_ONE = O.f32_to_bf16(np.ones(128, np.float32))
 
 
 def torch_():
