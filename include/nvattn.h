@@ -532,7 +532,8 @@ NVATTN_API nvattn_status nvattn_kv_load_q8(
  * context may hold anything.  A sequence of length 0 gives zeros.
  * NVATTN_ERR_UNSUPPORTED for batches whose bounds allow 2^30 key tiles (128
  * keys of a kv head) or more.  Results repeat bit for bit for a batch; another
- * batch composition splits a context elsewhere and may move the last bits.
+ * batch composition splits a context elsewhere and may move the last bits, and
+ * so may another max_context_len (it chooses the launch's CTAs per SM).
  * The launch uses the handle's workspace: calls on one handle are issued on
  * one stream, as for nvattn_paged_decode. */
 NVATTN_API nvattn_status nvattn_paged_decode_q8(

@@ -227,14 +227,14 @@ def make_handle(c, **kw):
     return handle(c["Hq"], c["Hkv"], nb, n_layer=nl, block_size=c["bs"], max_position=1, **kw)
 
 
-def run_decode(c, bf16=False, h=None, extra=1):
+def run_decode(c, bf16=False, h=None, extra=1, bound=None):
     torch = torch_()
     h = h or make_handle(c)
     q = to_q(c["q"], bf16)
     n = len(c["lens"])
     out = torch.full((n + extra,) + q.shape[1:], 7.0, dtype=q.dtype, device="cuda")
     h.decode_q8(c["layer"], q, *c["cache"].dev(), dev(c["bt"]), dev(c["lens"]),
-                int(c["lens"].max()), out[:n])
+                bound or int(c["lens"].max()), out[:n])
     torch.cuda.synchronize()
     assert (out[n:] == 7).all()  # rows behind the last sequence
     return h, out[:n].float().cpu().numpy(), q.float().cpu().numpy()
@@ -272,6 +272,24 @@ def test_decode_splits(cuda, lens, bs):
     h, got, q = run_decode(c)
     h.check_device()
     Q.check(got, *expect(c, q), False)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 8), (16, 8), (32, 8), (64, 8), (8, 1)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_decode_under_a_wide_bound(cuda, Hq, Hkv, bf16):
+    """The host's bound of the contexts chooses the launch (it takes a third CTA
+    per SM where the batch may be long); what it holds beyond the contexts, and
+    the table's columns there, change nothing but the last bits."""
+    c = decode_case(Hq + Hkv + 1, Hq, Hkv, EDGES + [6000], n_layer=2)
+    cols = 320 * 1024 // Hkv // c["bs"]
+    bound = cols * c["bs"]
+    c["bt"] = np.concatenate([c["bt"], np.full((len(c["lens"]), cols - c["bt"].shape[1]), -1,
+                                               np.int32)], 1)
+    h = make_handle(c, max_context=bound)
+    h, got, q = run_decode(c, bf16, h, bound=bound)
+    h.check_device()
+    Q.check(got, *expect(c, q), bf16)
+    assert np.array_equal(run_decode(c, bf16, h, bound=bound)[1], got)
 
 
 def test_decode_many_sequences(cuda):
