@@ -498,7 +498,7 @@ NVATTN_API nvattn_status nvattn_paged_tree_decode(
  * max|x| <= 448 s (E >= -100; s = 1 for a row of zeros), rounded to nearest
  * even; payload * s, the value every reader uses, is exact in bf16.  A row
  * that holds a NaN or an infinity is stored under a NaN scale and reads back
- * as NaN throughout. */
+ * as NaN throughout (e4m3's own NaN, 0x7f, is no payload of the format). */
 
 /* nvattn_kv_store_qk_norm_rope into the 8-bit cache: the same norm, rotation,
  * q_out and, where k_rows_f16_dev / v_rows_f16_dev are given (both or
@@ -528,7 +528,9 @@ NVATTN_API nvattn_status nvattn_kv_load_q8(
 
 /* nvattn_paged_decode over the 8-bit cache.  q_dev and out_dev are
  * [n_seqs][n_q_heads][head_dim] in dtype, f32 or bf16 (sums in f32 either
- * way; queries and softmax weights carry 22 bits).  Slots behind a sequence's
+ * way; queries carry 22 bits, and softmax weights 24 however small they are
+ * beside a row's largest: only a key whose weight times its V scale is below
+ * 2^-118 of the largest such product is left out).  Slots behind a sequence's
  * context may hold anything.  A sequence of length 0 gives zeros.
  * NVATTN_ERR_UNSUPPORTED for batches whose bounds allow 2^30 key tiles (128
  * keys of a kv head) or more.  Results repeat bit for bit for a batch; another

@@ -592,6 +592,11 @@ __device__ __forceinline__ uint64_t fsub2(uint64_t a, uint64_t b) {
   asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The next bf16 term of two values; they keep what is left.
+__device__ __forceinline__ void split_term(float& x0, float& x1, uint32_t& packed) {
+  packed = cvt_bf16x2(x0, x1);
+  unpack2(fsub2(pack2(x0, x1), pack2(bf16lo_to_f32(packed), bf16hi_to_f32(packed))), x0, x1);
+}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

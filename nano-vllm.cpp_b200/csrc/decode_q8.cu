@@ -8,15 +8,24 @@
 // score, and s_v joins the exponent,
 //   x_t = scale * log2(e) * s_k[t] * (q.K8[t]) + log2 s_v[t]
 //   w_t = 2^(x_t - M),  o = sum w_t V8[t] / sum w_t / s_v[t],  M >= x_t - 8
-// so that the weights handed to the tensor cores are at most 2^8 times the
-// row's reference whatever the rows' scales are.
+// A key with a large weight may add nothing to the output, or nothing to most
+// of its dims (a V row of zeros, which has scale 1; an attention sink with a
+// small V row; a row with one large dim), while it is the others, far below it,
+// that make the output.  So a weight keeps all of its bits however small it is
+// next to the largest: it goes to the tensor cores as a sum of three bf16
+// terms, 24 bits and f32's range.  (As an f16 value and its f16 remainder it had
+// an absolute floor of 2^-25: a zero row beside rows of size 0.01 cost the
+// output 8e-4 of its value, a zero row 12 nats above 9,000 others 0.3.)
 //
 // Bound by memory: 264 bytes per cached token and kv head against 2 * 128 * 2
 // products per query head.  The rows of one kv head are at most eight, so the
-// products run transposed as mma.sync m16n8k16 on f16 (which holds e4m3
-// exactly): tokens or dims in M, the query rows in N = 8, and queries and
-// weights as an f16 value and its f16 remainder (22 bits) in two products.  A
-// 128-row tcgen05 tile could not use its rows, and the 8-bit rows go from
+// products run transposed as mma.sync m16n8k16: tokens or dims in M, the query
+// rows in N = 8.  K's products are on f16 (which holds e4m3 exactly; one
+// conversion for two values), the queries as an f16 value and its f16 remainder
+// (22 bits); V's on bf16, where an e4m3 byte's exponent and mantissa, moved to
+// bf16's place, are its value times 2^-120 (subnormals included): a byte
+// permutation that extends the sign, a shift and a mask.  The weights carry 2^100
+// of that, so that products and sums stay normal, the output the rest.  A 128-row tcgen05 tile could not use its rows, and the 8-bit rows go from
 // shared memory through registers without the widened copy in shared memory
 // that a tcgen05 operand would need.
 //
@@ -114,6 +123,24 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte kI of two words of e4m3 values, as bf16 times 2^-120.
+template <int kI>
+__device__ __forceinline__ uint32_t e4m3_pair_to_bf16x2(uint32_t w0, uint32_t w1) {
+  constexpr uint32_t sel = kI | (8 + kI) << 4 | (4 + kI) << 8 | (12 + kI) << 12;  // 8: the sign
+  uint32_t t;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(t) : "r"(w0), "r"(w1), "n"(sel));
+  return (t << 4) & 0x87f087f0u;
+}
+constexpr float kWeightUp = 0x1p100f, kOutUp = 0x1p20f;  // together 2^120
 
 // Transposes an 8 x 8 matrix of 16-bit values, a row of four pairs per lane quad.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -527,17 +554,21 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e & 1];
         }
-        uint32_t wb[4][2];  // [eight tokens][weights, their remainders], as operands
+        uint32_t wb[4][3];  // [eight tokens][term of the weights], as operands
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           // (a step has a key: m is -inf only where every key's score is NaN)
-          const float w0 = fast_exp2(x[t][0] - m[0]), w1 = fast_exp2(x[t][1] - m[1]);
+          float w0 = fast_exp2(x[t][0] - m[0]), w1 = fast_exp2(x[t][1] - m[1]);
           l[0] = fmaf(w0, inv[t], l[0]);
           l[1] = fmaf(w1, inv[t], l[1]);
-          uint32_t hi, lo;
-          split_f16(w0, w1, hi, lo);
-          wb[t][0] = transpose8x8(hi);
-          wb[t][1] = transpose8x8(lo);
+          w0 *= kWeightUp;
+          w1 *= kWeightUp;
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            uint32_t term;
+            split_term(w0, w1, term);
+            wb[t][i] = transpose8x8(term);
+          }
         }
         // ---- o += V8 w ----
 #pragma unroll
@@ -550,16 +581,21 @@ __global__ void __launch_bounds__(kThreads, kCtas)
             v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a[2][4] = {{e4m3_pair_to_bf16x2<0>(v[0][i], v[1][i]),
+                                       e4m3_pair_to_bf16x2<1>(v[0][i], v[1][i]),
+                                       e4m3_pair_to_bf16x2<0>(v[2][i], v[3][i]),
+                                       e4m3_pair_to_bf16x2<1>(v[2][i], v[3][i])},
+                                      {e4m3_pair_to_bf16x2<2>(v[0][i], v[1][i]),
+                                       e4m3_pair_to_bf16x2<3>(v[0][i], v[1][i]),
+                                       e4m3_pair_to_bf16x2<2>(v[2][i], v[3][i]),
+                                       e4m3_pair_to_bf16x2<3>(v[2][i], v[3][i])}};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t t0 = __byte_perm(v[0][i], v[1][i], h ? 0x7362 : 0x5140);
-              const uint32_t t1 = __byte_perm(v[2][i], v[3][i], h ? 0x7362 : 0x5140);
-              const uint32_t a[4] = {e4m3x2_to_f16x2(t0 & 0xffffu), e4m3x2_to_f16x2(t0 >> 16),
-                                     e4m3x2_to_f16x2(t1 & 0xffffu), e4m3x2_to_f16x2(t1 >> 16)};
-              mma_f16(o[2 * i + h], a, wb[2 * ks][0], wb[2 * ks + 1][0]);
-              mma_f16(o[2 * i + h], a, wb[2 * ks][1], wb[2 * ks + 1][1]);
-            }
+            for (int term = 2; term >= 0; --term)  // the small terms first
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                mma_bf16(o[2 * i + h], a[h], wb[2 * ks][term], wb[2 * ks + 1][term]);
+          }
         }
         __syncwarp();  // every lane has read the stage
       }
@@ -591,7 +627,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         rows[(2 * c + r) * (kD / 4) + merge_chunk(2 * c + r, 4 * pr + j)] =
-            make_float4(o[2 * j][r], o[2 * j][2 + r], o[2 * j + 1][r], o[2 * j + 1][2 + r]);
+            make_float4(o[2 * j][r] * kOutUp, o[2 * j][2 + r] * kOutUp,
+                        o[2 * j + 1][r] * kOutUp, o[2 * j + 1][2 + r] * kOutUp);
     __syncthreads();
     for (int r = warp; r < p.G; r += kWarps) {
       float M = -INFINITY, L = 0.0f;

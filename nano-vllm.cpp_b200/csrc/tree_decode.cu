@@ -190,12 +190,6 @@ struct Walker {
   }
 };
 
-// The next bf16 term of two values; they keep what is left.
-__device__ __forceinline__ void split_term(float& x0, float& x1, uint32_t& packed) {
-  packed = cvt_bf16x2(x0, x1);
-  unpack2(fsub2(pack2(x0, x1), pack2(bf16lo_to_f32(packed), bf16hi_to_f32(packed))), x0, x1);
-}
-
 // kN consecutive dims of an output row at element `at`, times f.
 template <bool kF32, int kN>
 __device__ __forceinline__ void write_dims(const TreeParams& p, long long at, const float (&o)[kN],
