@@ -528,9 +528,10 @@ NVATTN_API nvattn_status nvattn_kv_load_q8(
 
 /* nvattn_paged_decode over the 8-bit cache.  q_dev and out_dev are
  * [n_seqs][n_q_heads][head_dim] in dtype, f32 or bf16 (sums in f32 either
- * way; queries carry 22 bits, and softmax weights 24 however small they are
- * beside a row's largest: only a key whose weight times its V scale is below
- * 2^-118 of the largest such product is left out).  Slots behind a sequence's
+ * way; f32 queries carry 22 bits, down to 2^-28 of their row's largest, and
+ * softmax weights 24 however small they are beside the row's others: only a
+ * key whose weight times its V scale is below 2^-118 of the largest such
+ * product is left out).  Slots behind a sequence's
  * context may hold anything.  A sequence of length 0 gives zeros.
  * NVATTN_ERR_UNSUPPORTED for batches whose bounds allow 2^30 key tiles (128
  * keys of a kv head) or more.  Results repeat bit for bit for a batch; another

@@ -21,8 +21,10 @@
 // products per query head.  The rows of one kv head are at most eight, so the
 // products run transposed as mma.sync m16n8k16: tokens or dims in M, the query
 // rows in N = 8.  K's products are on f16 (which holds e4m3 exactly; one
-// conversion for two values), the queries as an f16 value and its f16 remainder
-// (22 bits); V's on bf16, where an e4m3 byte's exponent and mantissa, moved to
+// conversion for two values), the queries scaled to f16's upper range: bf16 ones
+// are f16 values then, f32 ones a value and its remainder times 2^11, whose
+// products are summed apart (22 bits of a query down to 2^-28 of its row's
+// largest); V's on bf16, where an e4m3 byte's exponent and mantissa, moved to
 // bf16's place, are its value times 2^-120 (subnormals included): a byte
 // permutation that extends the sign, a shift and a mask.  The weights carry 2^100
 // of that, so that products and sums stay normal, the output the rest.  A 128-row tcgen05 tile could not use its rows, and the 8-bit rows go from
@@ -149,14 +151,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-// hi = f16(x), lo = f16(x - hi) of two values, packed.
+// hi = f16(x), lo = f16(kRestUp (x - hi)) of two values, packed.
+constexpr float kRestUp = 0x1p11f;
 __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
   hi = cvt_f16x2(x0, x1);
   float h0, h1;
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
       : "=f"(h0), "=f"(h1)
       : "r"(hi));
-  lo = cvt_f16x2(x0 - h0, x1 - h1);
+  lo = cvt_f16x2((x0 - h0) * kRestUp, (x1 - h1) * kRestUp);
 }
 
 // Where a walk over the CTA's run of tiles stands.
@@ -197,11 +200,15 @@ __device__ __forceinline__ void walk_next(const Q8Params& p, int end, Walk& w) {
 }
 
 // The query rows of (seq, head) as mma operands: row g scaled by a power of two
-// so that max|q| lies in [1, 2); a[k] = {first pair hi, lo, second pair hi, lo}.
+// so that max|q| lies in [2^14, 2^15); a[k] = {first pair, second pair}, and for
+// f32 queries their remainders.  (A bf16 value has 8 bits, so it is an f16 one
+// down to 2^-28 of the row's largest, and below that off by 2^-39 of it.)
 // Returns the factor that undoes the scaling (of row g).
 template <bool kBf16>
+constexpr int kQWords = kBf16 ? 2 : 4;
+template <bool kBf16>
 __device__ __forceinline__ float load_q(const Q8Params& p, int seq, int head, int g, int c,
-                                        uint32_t (&a)[8][4]) {
+                                        uint32_t (&a)[8][kQWords<kBf16>]) {
   float x[2][16];
   const bool real = g < p.G;
   const long long off = ((long long)seq * p.Hq + (long long)head * p.G + g) * kD + 16 * c;
@@ -240,15 +247,20 @@ __device__ __forceinline__ float load_q(const Q8Params& p, int seq, int head, in
   big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
   big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
   int e = (int)(big >> 23) - 127;
-  e = (big == 0 || big >= 0x7f800000u) ? 0 : min(max(e, -100), 100);
+  e = (big == 0 || big >= 0x7f800000u) ? 0 : max(e - 14, -126);
   const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t* f = a[4 * hf + i];
-      split_f16(x[hf][4 * i] * down, x[hf][4 * i + 1] * down, f[0], f[1]);
-      split_f16(x[hf][4 * i + 2] * down, x[hf][4 * i + 3] * down, f[2], f[3]);
+      if constexpr (kBf16) {
+        f[0] = cvt_f16x2(x[hf][4 * i] * down, x[hf][4 * i + 1] * down);
+        f[1] = cvt_f16x2(x[hf][4 * i + 2] * down, x[hf][4 * i + 3] * down);
+      } else {
+        split_f16(x[hf][4 * i] * down, x[hf][4 * i + 1] * down, f[0], f[2]);
+        split_f16(x[hf][4 * i + 2] * down, x[hf][4 * i + 3] * down, f[1], f[3]);
+      }
     }
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
@@ -446,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   // (`ahead` may run past the last tile by the ring's depth: no step there)
   for (int i = 0; i < kStages && ahead.at < run.end; ++i) issue();
 
-  uint32_t qa[8][4];
+  uint32_t qa[8][kQWords<kBf16>];
   float o[8][4];  // [j]: dims 16 ch + 2 j (elements 0, 1: rows 2c, 2c + 1) and 2 j + 1 (2, 3)
   const int pr = (g >> 1) | ((g & 1) << 2);
 
@@ -519,9 +531,9 @@ __global__ void __launch_bounds__(kThreads, kCtas)
                                      e4m3x2_to_f16x2(u[2 * mt + 1][i] & 0xffffu),
                                      e4m3x2_to_f16x2(u[2 * mt][i] >> 16),
                                      e4m3x2_to_f16x2(u[2 * mt + 1][i] >> 16)};
-              const uint32_t(&q)[4] = qa[4 * hf + i];
-              mma_f16(s[mt][0], a, q[0], q[2]);
-              mma_f16(s[mt][1], a, q[1], q[3]);
+              const uint32_t* q = qa[4 * hf + i];
+              mma_f16(s[mt][0], a, q[0], q[1]);
+              if constexpr (!kBf16) mma_f16(s[mt][1], a, q[2], q[3]);
             }
         }
         float x[4][2], inv[4];  // [eight tokens][query row]
@@ -529,8 +541,12 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         for (int t = 0; t < 4; ++t) {
           const float4 f = sm.tok[warp][8 * t + pr];
           const int mt = t >> 1, e = 2 * (t & 1);
-          x[t][0] = fmaf((s[mt][0][e] + s[mt][1][e]) * up[0], f.x, f.y);
-          x[t][1] = fmaf((s[mt][0][e + 1] + s[mt][1][e + 1]) * up[1], f.x, f.y);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float y = s[mt][0][e + r];
+            if constexpr (!kBf16) y = fmaf(s[mt][1][e + r], 1.0f / kRestUp, y);
+            x[t][r] = fmaf(y * up[r], f.x, f.y);
+          }
           inv[t] = f.z;
         }
         float top[2];
