@@ -156,10 +156,14 @@ __device__ __forceinline__ void load_tile(const Args& a, const void* row, int ti
 }
 
 // Sums under a new reference (m_new >= a.m; -infinity: nothing summed yet).
+// The step between them counts as -1e4 at most, where its factor is 0 already:
+// from a tile masked with the type's lowest value it would overflow beside s,
+// and 0 * -infinity is NaN.
 __device__ __forceinline__ void rescale(float m, float m_new, float& s, float& t) {
   if (m_new == m || m == -INFINITY) return;
-  const float f = fast_exp2((m - m_new) * kLog2e);
-  t = f * fmaf(m - m_new, s, t);
+  const float d = fmaxf(m - m_new, -1.0e4f);
+  const float f = fast_exp2(d * kLog2e);
+  t = f * fmaf(d, s, t);
   s *= f;
 }
 
