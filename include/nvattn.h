@@ -249,7 +249,8 @@ NVATTN_API nvattn_status nvattn_sample(
  * NVATTN_ERR_OUT_OF_RANGE (detail = r), its row's logprob is NaN and its rank
  * -1.  In the order a NaN counts as -inf and -0 equals +0; a row with a NaN, a
  * +inf or nothing but -inf has NaN log-probabilities and entropy, as the
- * formulas give.  n_vocab <= 2,097,152.  One launch, no workspace. */
+ * formulas give.  n_vocab <= 2,097,152.  One launch per 65,535 rows, no
+ * workspace. */
 NVATTN_API nvattn_status nvattn_token_logprobs(
     nvattn_handle* h, int n_rows, int n_vocab, const void* logits_dev, nvattn_dtype dtype,
     int64_t row_stride, const int32_t* tokens_dev, float* logprobs_dev, float* entropy_dev,

@@ -50,6 +50,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
   int n_vocab, top_k;
+  int row0;  // the launch's first row of the call
   long long row_stride;
   const void* logits;
   const int32_t* tokens;
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(Args a) {
     sm.log_s = log_s;
     if (a.entropy != nullptr) a.entropy[row_i] = log_s - w.t / w.s;
     if (a.tokens != nullptr) {
-      if (!has_token) record_error(a.status, NVATTN_ERR_OUT_OF_RANGE, 95, row_i);
+      if (!has_token) record_error(a.status, NVATTN_ERR_OUT_OF_RANGE, 95, a.row0 + row_i);
       if (a.logprobs != nullptr) a.logprobs[row_i] = raw_xt - m - log_s;
       if (a.ranks != nullptr) a.ranks[row_i] = has_token ? w.before : -1;
     }
@@ -459,6 +460,7 @@ nvattn_status launch_token_logprobs(nvattn_handle* h, int n_rows, int n_vocab, c
   for (int r0 = 0; r0 < n_rows; r0 += kMaxRowsPerLaunch) {
     const int n = std::min(n_rows - r0, kMaxRowsPerLaunch);
     cfg.gridDim = dim3(cluster, n);
+    a.row0 = r0;
     if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return NVATTN_ERR_CUDA;
     a.logits = static_cast<const char*>(a.logits) + (long long)n * row_stride * el;
     if (a.tokens) a.tokens += n;
