@@ -499,7 +499,8 @@ NVATTN_API nvattn_status nvattn_paged_tree_decode(
  * max|x| <= 448 s (E >= -100; s = 1 for a row of zeros), rounded to nearest
  * even; payload * s, the value every reader uses, is exact in bf16.  A row
  * that holds a NaN or an infinity is stored under a NaN scale and reads back
- * as NaN throughout (e4m3's own NaN, 0x7f, is no payload of the format). */
+ * as NaN throughout (e4m3's own NaN, 0x7f, is no payload of the format).
+ * Arrays that begin as zeros hold rows of zeros. */
 
 /* nvattn_kv_store_qk_norm_rope into the 8-bit cache: the same norm, rotation,
  * q_out and, where k_rows_f16_dev / v_rows_f16_dev are given (both or

@@ -489,10 +489,12 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         // ---- the tokens' factors ----
         {
           const float sk = sm.ks[warp][st][lane], sv = sm.vs[warp][st][lane];
-          const uint32_t b = __float_as_uint(sv);
-          // a NaN scale (a row that held a NaN or an infinity) stays NaN
-          float4 f = make_float4(sk * p.scale_log2, (float)((int)(b >> 23) - 127) + (sv - sv),
-                                 __uint_as_float((254u << 23) - (b & 0x7f800000u)), 0.0f);
+          // A NaN scale (a row that held a NaN or an infinity) stays NaN; a scale
+          // of 0 (a row never written in a cache that began as zeros) counts as the
+          // least one, 2^-100: its reciprocal would be 2^127, two of which overflow.
+          const uint32_t e = max(__float_as_uint(sv) >> 23, 27u);
+          float4 f = make_float4(sk * p.scale_log2, (float)((int)e - 127) + (sv - sv),
+                                 __uint_as_float((254u - e) << 23), 0.0f);
           if (lane >= n) {
             // Slots behind the context hold anything: weight zero, and rows
             // of zeros so that no NaN meets it.

@@ -146,7 +146,7 @@ class DecodeRunner:
             pages = (shape.n_layer, num_blocks, shape.n_kv_heads, BS)
             self.q8_cache = [t for _ in "kv" for t in (
                 torch.zeros(pages + (shape.head_dim,), dtype=torch.uint8, device=device),
-                torch.zeros(pages, device=device))]
+                torch.ones(pages, device=device))]  # rows of zeros, in the format
         else:
             self.k_cache = torch.zeros((shape.n_layer, n_slots, shape.n_kv_heads, shape.head_dim),
                                        dtype=torch.int16, device=device)
