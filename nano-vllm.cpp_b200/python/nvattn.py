@@ -205,6 +205,32 @@ class _Dtypes(dict):
 
 
 _DTYPES = _Dtypes()
+MAX_TOP = 64  # nvattn_token_logprobs' largest top_k
+
+
+class _Words:
+    """The element types that cross the ABI as they are, known after the first
+    call of _check_words (torch is not imported before)."""
+    i32 = f32 = None
+
+
+def _check_words(ints, floats):
+    """Refuses integers that are not int32 and values that are not f32: the
+    kernels would read another type as wrong numbers.  (The methods compare the
+    types in place and come here at the first call, or to raise.)"""
+    import torch
+    _Words.i32, _Words.f32 = torch.int32, torch.float32
+    for want, tensors in ((torch.int32, ints), (torch.float32, floats)):
+        for t in tensors:
+            if t is not None and t.dtype is not want:
+                raise TypeError(f"expected {want}, got {t.dtype}")
+
+
+def _check_q8_cache(k_q8, k_scale, v_q8, v_scale):
+    if k_q8.element_size() != 1 or v_q8.element_size() != 1:
+        raise TypeError("an 8-bit cache's payload has one byte per value")
+    if k_scale.dtype is not _Words.f32 or v_scale.dtype is not _Words.f32:
+        _check_words((), (k_scale, v_scale))
 
 
 class Handle:
@@ -388,6 +414,12 @@ class Handle:
             raise ValueError("q and out differ in type")
         if tree_mask.element_size() != 8 or tree_mask.shape[0] < q.shape[0]:
             raise ValueError("tree_mask holds 64-bit words, a row per node")
+        i32 = _Words.i32
+        if cu_nodes.dtype is not i32 or block_tables.dtype is not i32 or \
+                context_lens.dtype is not i32:
+            _check_words((cu_nodes, block_tables, context_lens), ())
+        if k_cache.element_size() != 2 or v_cache.element_size() != 2:
+            raise TypeError("the cache is BF16")
         st = self._L.nvattn_paged_tree_decode(
             self._h, layer, context_lens.shape[0], q.shape[0], q.data_ptr(), _DTYPES[q.dtype],
             cu_nodes.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], int(max_nodes),
@@ -401,14 +433,29 @@ class Handle:
     def token_logprobs(self, logits, tokens=None, logprobs=None, entropy=None, ranks=None,
                        top_ids=None, top_logprobs=None, stream=None, check=True):
         """nvattn_token_logprobs: logits [n_rows][n_vocab] f32 or bf16 with
-        unit stride along the vocabulary; top_k is top_ids.shape[1]."""
+        unit stride along the vocabulary; tokens, ranks and top_ids int32, the
+        other outputs f32; top_k is top_ids.shape[1]."""
         n, V = logits.shape
         if V > 1 and logits.stride(1) != 1:
             raise ValueError("logits are not contiguous along the vocabulary")
+        i32, f32 = _Words.i32, _Words.f32
+        if (tokens is not None and tokens.dtype is not i32) or \
+                (ranks is not None and ranks.dtype is not i32) or \
+                (logprobs is not None and logprobs.dtype is not f32) or \
+                (entropy is not None and entropy.dtype is not f32):
+            _check_words((tokens, ranks), (logprobs, entropy))
+        top_k = 0
+        if top_ids is not None:
+            top_k = top_ids.size(1)
+            if top_logprobs is not None:
+                if top_ids.dtype is not i32 or top_logprobs.dtype is not f32:
+                    _check_words((top_ids,), (top_logprobs,))
+                if top_logprobs.size(1) != top_k <= MAX_TOP:
+                    raise ValueError("top_ids and top_logprobs differ in their columns")
         st = self._L.nvattn_token_logprobs(
             self._h, n, V, _addr(logits), _DTYPES[logits.dtype], logits.stride(0) if n > 1 else V,
             _addr(tokens), _addr(logprobs), _addr(entropy), _addr(ranks),
-            0 if top_ids is None else top_ids.shape[1], _addr(top_ids), _addr(top_logprobs),
+            top_k, _addr(top_ids), _addr(top_logprobs),
             _stream_addr(stream))
         if check:
             _check(st, "nvattn_token_logprobs")
@@ -419,6 +466,9 @@ class Handle:
     def kv_store_q8(self, layer, q, k, v, q_norm_w, k_norm_w, positions, slots, q_out, k_q8,
                     k_scale, v_q8, v_scale, stream=None, check=True, k_rows=None, v_rows=None):
         """nvattn_kv_store_q8: kv_store into the 8-bit cache."""
+        if positions.dtype is not _Words.i32 or slots.dtype is not _Words.i32:
+            _check_words((positions, slots), ())
+        _check_q8_cache(k_q8, k_scale, v_q8, v_scale)
         st = self._L.nvattn_kv_store_q8(
             self._h, layer, positions.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(),
             q_norm_w.data_ptr(), k_norm_w.data_ptr(), positions.data_ptr(), slots.data_ptr(),
@@ -436,6 +486,9 @@ class Handle:
         dtype = k_out.dtype
         if v_out.dtype != dtype:
             raise ValueError("k_out and v_out differ in type")
+        if slots.dtype is not _Words.i32:
+            _check_words((slots,), ())
+        _check_q8_cache(k_q8, k_scale, v_q8, v_scale)
         st = self._L.nvattn_kv_load_q8(
             self._h, layer, slots.shape[0], slots.data_ptr(), k_q8.data_ptr(), k_scale.data_ptr(),
             v_q8.data_ptr(), v_scale.data_ptr(), _DTYPES[dtype], k_out.data_ptr(),
@@ -450,6 +503,9 @@ class Handle:
         dtype = q.dtype
         if out.dtype != dtype:
             raise ValueError("q and out differ in type")
+        if block_tables.dtype is not _Words.i32 or context_lens.dtype is not _Words.i32:
+            _check_words((block_tables, context_lens), ())
+        _check_q8_cache(k_q8, k_scale, v_q8, v_scale)
         st = self._L.nvattn_paged_decode_q8(
             self._h, layer, context_lens.shape[0], q.data_ptr(), _DTYPES[dtype], k_q8.data_ptr(),
             k_scale.data_ptr(), v_q8.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
