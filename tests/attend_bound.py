@@ -13,14 +13,16 @@ Per score (in nats; size = sum |q k|, big = max |q k|, both times the scale):
 Per weight: the exponential 2^-22, up to eight factors 2^-22 where references move
 and partials meet, and the weights' representation, 2^-w_bits.
 Per output: accumulations of 16 weighted rows, in three terms, by a chain of up to
-a fourth of the keys and 32 more for merges, 2^-23 of sum p |v| each; the sum of
-weights, n / 16 + 40 additions of 2^-24."""
+a fourth of the keys (steps = 3 of them for 64 keys; the tree kernel's two groups
+take half of the keys each: 6) and 32 more for merges, 2^-23 of sum p |v| each; the
+sum of weights, n / 16 + 40 additions of 2^-24."""
 import numpy as np
 
 D = 128
 
 
-def attend(q, k, v, keep=None, s_v=None, scale=1 / np.sqrt(D), q_bits=22, w_bits=23):
+def attend(q, k, v, keep=None, s_v=None, scale=1 / np.sqrt(D), q_bits=22, w_bits=23,
+           steps=3):
     """Rows q [R][128] over keys [n][128]; keep [R][n] masks, s_v [n] the power-of-two
     scales of the V rows.  Returns the output and its bound, [R][128]."""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
@@ -43,5 +45,5 @@ def attend(q, k, v, keep=None, s_v=None, scale=1 / np.sqrt(D), q_bits=22, w_bits
     out, each = p @ v, p @ np.abs(v)
     tol = ((p * rel) @ np.abs(v) + np.abs(out) * ((p * rel).sum(-1, keepdims=True) +
                                                   (n / 16 + 40) * 2.0 ** -24) +
-           (3 * np.ceil(n / 64) + 32) * 2.0 ** -23 * each)
+           (steps * np.ceil(n / 64) + 32) * 2.0 ** -23 * each)
     return out, tol
