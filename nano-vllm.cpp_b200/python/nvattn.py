@@ -188,7 +188,8 @@ def _addr(t):
 def _stream_addr(stream):
     if stream is None:
         return None
-    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+    addr = getattr(stream, "cuda_stream", None)
+    return int(stream) if addr is None else addr
 
 
 class _Dtypes(dict):
@@ -226,11 +227,12 @@ def _check_words(ints, floats):
                 raise TypeError(f"expected {want}, got {t.dtype}")
 
 
-def _check_q8_cache(k_q8, k_scale, v_q8, v_scale):
-    if k_q8.element_size() != 1 or v_q8.element_size() != 1:
-        raise TypeError("an 8-bit cache's payload has one byte per value")
-    if k_scale.dtype is not _Words.f32 or v_scale.dtype is not _Words.f32:
+def _check_q8_cache(k_q8, k_scale, v_q8, v_scale, words=_Words):
+    f32 = words.f32
+    if k_scale.dtype is not f32 or v_scale.dtype is not f32:
         _check_words((), (k_scale, v_scale))
+    if k_q8.itemsize != 1 or v_q8.itemsize != 1:
+        raise TypeError("an 8-bit cache's payload has one byte per value")
 
 
 class Handle:
@@ -446,11 +448,11 @@ class Handle:
             _check_words((tokens, ranks), (logprobs, entropy))
         top_k = 0
         if top_ids is not None:
-            top_k = top_ids.size(1)
+            top_k = top_ids.shape[1]
             if top_logprobs is not None:
                 if top_ids.dtype is not i32 or top_logprobs.dtype is not f32:
                     _check_words((top_ids,), (top_logprobs,))
-                if top_logprobs.size(1) != top_k <= MAX_TOP:
+                if top_logprobs.shape[1] != top_k <= MAX_TOP:
                     raise ValueError("top_ids and top_logprobs differ in their columns")
         st = self._L.nvattn_token_logprobs(
             self._h, n, V, _addr(logits), _DTYPES[logits.dtype], logits.stride(0) if n > 1 else V,
