@@ -90,7 +90,8 @@ nvattn_status get_cache_tensor_map(nvattn_handle* h, const void* base, int box_d
                                    int swizzle, CUtensorMap* out) {
   for (int i = 0; i < h->n_maps; ++i) {
     const NvattnTensorMapEntry& e = h->maps[i];
-    if (e.kind == kMapCache && e.base == base && e.box_d == box_d && e.box_rows == box_rows && e.swizzle == swizzle) {
+    if (e.kind == kMapCache && e.base == base && e.box_d == box_d && e.box_rows == box_rows &&
+        e.swizzle == swizzle) {
       *out = e.map;
       return NVATTN_OK;
     }

@@ -600,10 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool special = col0 + kT > first;  // the tile holds nodes (or keys past the end)
         uint64_t allowed = 0;                    // which of its keys the row attends
         if (special) {  // (before the wait for its scores, which it hides behind)
-          const int rel = col0 - first;  // the first key's place among the nodes
-          if (rel <= -kT) {
-            allowed = ~0ull;
-          } else if (real) {
+          const int rel = col0 - first;  // the first key's place among the nodes, > -kT
+          if (real) {
             const uint64_t* words = p.mask + (long long)node * p.mask_words;
             if (rel < 0) {
               allowed = (words[0] << -rel) | ((1ull << -rel) - 1);
