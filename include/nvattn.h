@@ -466,10 +466,11 @@ NVATTN_API nvattn_status nvattn_paged_prefill_rows(
  *   cu_nodes_dev [n_seqs+1] int32, tree_mask_dev [n_nodes][mask_words] uint64,
  *       1 <= mask_words <= 4, max_nodes (host bound of N_s) <= 64 * mask_words
  *   the rest as nvattn_paged_decode
- * A node that attends nothing gets zeros.  Slots behind a context may hold
- * anything, and so may the K/V rows of a node that no mask names: a node's K/V
- * reaches only the rows that attend it (a NaN or an infinity in its V row
- * makes all of their output NaN).  A sequence without nodes is skipped; one
+ * A node that attends nothing gets zeros.  V values are at most 2^70 in size
+ * (the sums carry weights of up to 2^32 until they are divided out).  Slots
+ * behind a context may hold anything, and so may the K/V rows of a node that no
+ * mask names: a node's K/V reaches only the rows that attend it (a NaN or an
+ * infinity in its V row makes all of their output NaN).  A sequence without nodes is skipped; one
  * whose cu_nodes or context_lens are unusable (N_s negative or above max_nodes,
  * rows outside n_nodes, context_lens[s] outside [N_s, max_context_len]) is
  * reported as NVATTN_ERR_OUT_OF_RANGE and its rows are not written.

@@ -13,23 +13,27 @@
 // small V row; a row with one large dim), while it is the others, far below it,
 // that make the output.  So a weight keeps all of its bits however small it is
 // next to the largest: it goes to the tensor cores as a sum of three bf16
-// terms, 24 bits and f32's range.  (As an f16 value and its f16 remainder it had
-// an absolute floor of 2^-25: a zero row beside rows of size 0.01 cost the
-// output 8e-4 of its value, a zero row 12 nats above 9,000 others 0.3.)
+// terms, 24 bits and f32's range.  (As an f16 value and its f16 remainder, two
+// products instead of three, it had an absolute floor of 2^-25: a zero row
+// beside rows of size 0.01 cost the output 8e-4 of its value, a zero row 12 nats
+// above 9,000 others 0.3.  The third product costs 10 of the 156 us of 64 long
+// f32 sequences, the bf16 operands 7.)
 //
-// Bound by memory: 264 bytes per cached token and kv head against 2 * 128 * 2
-// products per query head.  The rows of one kv head are at most eight, so the
-// products run transposed as mma.sync m16n8k16: tokens or dims in M, the query
-// rows in N = 8.  K's products are on f16 (which holds e4m3 exactly; one
-// conversion for two values), the queries scaled to f16's upper range: bf16 ones
-// are f16 values then, f32 ones a value and its remainder times 2^11, whose
-// products are summed apart (22 bits of a query down to 2^-28 of its row's
-// largest); V's on bf16, where an e4m3 byte's exponent and mantissa, moved to
-// bf16's place, are its value times 2^-120 (subnormals included): a byte
-// permutation that extends the sign, a shift and a mask.  The weights carry 2^100
-// of that, so that products and sums stay normal, the output the rest.  A 128-row tcgen05 tile could not use its rows, and the 8-bit rows go from
+// Bound by memory (264 bytes per cached token and kv head against 2 * 128 * 2
+// products per query head), and near it by the chain of a step's products and
+// exponentials.  The rows of one kv head are at most eight, so the products run
+// transposed as mma.sync m16n8k16: tokens or dims in M, the query rows in N = 8.
+// A 128-row tcgen05 tile could not use its rows, and the 8-bit rows go from
 // shared memory through registers without the widened copy in shared memory
 // that a tcgen05 operand would need.
+//   K: f16, which holds e4m3 exactly, one conversion for two values.  The
+//      queries are scaled to f16's upper range: bf16 ones are f16 values then,
+//      f32 ones a value and its remainder times 2^11, whose products are summed
+//      apart (22 bits of a query down to 2^-28 of its row's largest).
+//   V: bf16, where an e4m3 byte's exponent and mantissa, moved to bf16's place,
+//      are its value times 2^-120 (subnormals included): a byte permutation that
+//      extends the sign, a shift and a mask.  The weights make up for 2^100 of
+//      that, so that products and sums stay normal, the output for the rest.
 //
 // Each warp works alone: 32-token steps, K and V tiles of 4 KiB each by TMA
 // (128-byte swizzle) and their scales by bulk copies into its own ring of
@@ -68,8 +72,8 @@ static_assert(kRows == 2 * kWarps, "merge_parts: two rows per warp");
 // cost about as much as this many tiles, and the split counts them as such.
 constexpr int kUnitCost = 2;
 // Three CTAs per SM hide more of a warp's own latencies (64 sequences of 1k to
-// 16k tokens: 139 us, two: 145), two make fewer partials and merges (24 ragged
-// batches of 10 to 30 us: 3.5 % less in the mean).  Three where the batch may
+// 16k tokens, f32: 156 us, two: 164), two make fewer partials and merges (24 ragged
+// batches of 10 to 35 us: 5 to 8 % less in the mean).  Three where the batch may
 // hold so many tiles per CTA, by the host's bound of the contexts.
 constexpr int kFullGridTiles = 48;
 // Shared memory of a launch with two CTAs per SM: more than a third of an SM's,
